@@ -336,6 +336,122 @@ size_t ttj_block_workspace_size(int64_t batch, int64_t seq_len, int64_t d_model,
  */
 int ttj_transformer_block_fwd(const ttj_block_args* args, ttj_stream_t stream);
 
+/* ------------------------------------------------------------- serving: prompts, caches */
+
+/*
+ * Grouped heads: num_heads query heads share num_kv_heads key / value heads;
+ * query head h reads key / value head h / group, group = num_heads /
+ * num_kv_heads (at most 128).  head_dim as above (a multiple of 8 up to 256).
+ * Tensors of these entry points carry element strides for every dimension but
+ * the innermost, which is contiguous; strides and base addresses are multiples
+ * of 16 bytes.
+ *
+ * Work plan of a packed batch of prompts.  seq_lens (a HOST array, entries may
+ * be zero) lists the prompts' lengths in the order they are packed.  The plan
+ * is an array of ttj_prompt_plan_entries() records of four int32 that
+ * ttj_prompt_plan_build() writes to HOST memory; the caller copies it to the
+ * device once and every layer's ttj_prompt_attn_fwd reads it.  A negative
+ * result is a ttj_status.
+ */
+int64_t ttj_prompt_plan_entries(const int64_t* seq_lens, int64_t num_seqs, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim);
+int ttj_prompt_plan_build(const int64_t* seq_lens, int64_t num_seqs, int64_t num_heads,
+                          int64_t num_kv_heads, int64_t head_dim, int32_t* plan,
+                          int64_t plan_entries);
+
+/* Arguments of causal attention over packed prompts. */
+typedef struct ttj_prompt_attn_args {
+  const void* q;                   /* [T, num_heads, head_dim] */
+  const void* k;                   /* [T, num_kv_heads, head_dim] */
+  const void* v;                   /* [T, num_kv_heads, head_dim] */
+  void* out;                       /* [T, num_heads, head_dim] contiguous; aliases no input */
+  float* lse;                      /* [T, num_heads] log of each row's sum of exponentials, or NULL */
+  const int32_t* plan;             /* DEVICE copy of the plan */
+  int64_t plan_entries;
+  int* status;                     /* device status word or NULL */
+  int64_t tokens, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  float scale;                     /* of the scores, e.g. head_dim^-0.5; positive */
+  int dtype;                       /* TTJ_F16 or TTJ_BF16 */
+} ttj_prompt_attn_args;
+
+/*
+ * out[t,h] = sum over the tokens u <= t of t's own prompt of p[t,u] v[u, h/group],
+ * p[t,:] = softmax(scale * q[t,h] . k[u, h/group]).  fp32 statistics; the
+ * probabilities are rounded to `dtype` for the product with v, as in
+ * ttj_flash_attn_fwd.  Tokens of other prompts are not read into a row's
+ * result whatever they hold (infinities and NaN included).
+ */
+int ttj_prompt_attn_fwd(const ttj_prompt_attn_args* args, ttj_stream_t stream);
+
+/* Arguments of one decode step over a shared prefix and per-sequence caches. */
+typedef struct ttj_shared_prefix_attn_args {
+  const void* q;                   /* [B, num_heads, head_dim], one new token per sequence */
+  const void* prefix_k;            /* [P, num_kv_heads, head_dim]; unused when P == 0 */
+  const void* prefix_v;
+  const void* k_cache;             /* [B, C, num_kv_heads, head_dim]; unused when C == 0 */
+  const void* v_cache;
+  const int32_t* lengths;          /* [B] used rows of each cache (clamped to 0..C) */
+  const float* key_weights;        /* [B, num_kv_heads, C] or NULL */
+  float* key_weights_out;          /* same shape, aliases no input; required with key_weights */
+  void* out;                       /* [B, num_heads, head_dim] contiguous */
+  void* workspace;
+  size_t workspace_bytes;
+  int* status;
+  int64_t batch, prefix_len, capacity, num_heads, num_kv_heads, head_dim;
+  int64_t q_seq_stride, q_head_stride;
+  int64_t prefix_k_row_stride, prefix_k_head_stride;
+  int64_t prefix_v_row_stride, prefix_v_head_stride;
+  int64_t k_seq_stride, k_row_stride, k_head_stride;
+  int64_t v_seq_stride, v_row_stride, v_head_stride;
+  float scale;
+  int dtype;
+} ttj_shared_prefix_attn_args;
+
+size_t ttj_shared_prefix_attn_workspace_size(int64_t batch, int64_t prefix_len, int64_t capacity,
+                                             int64_t num_heads, int64_t num_kv_heads,
+                                             int64_t head_dim, int with_key_weights);
+
+/*
+ * Sequence b's token attends the P prefix rows (the same for the whole batch,
+ * read once for all) and then rows 0 .. lengths[b]-1 of its own cache; a
+ * sequence with no key at all gets zeros.  With key_weights,
+ *   key_weights_out[b,j,c] = key_weights[b,j,c] + sum over the group's heads of
+ *                            this step's probability of cache row c
+ * for c < lengths[b], and key_weights[b,j,c] for the rows beyond.  Cache rows
+ * at and past the length may hold anything.
+ */
+int ttj_shared_prefix_attn_fwd(const ttj_shared_prefix_attn_args* args, ttj_stream_t stream);
+
+/* Arguments of the eviction from per-sequence caches. */
+typedef struct ttj_cache_evict_args {
+  const void* k_cache;             /* [B, C, num_kv_heads, head_dim], 16-bit elements */
+  const void* v_cache;
+  const float* key_weights;        /* [B, num_kv_heads, C] */
+  const int32_t* lengths;          /* [B] (clamped to 0..C) */
+  void* k_out;                     /* [B, budget, num_kv_heads, head_dim]; aliases no input */
+  void* v_out;
+  float* weights_out;              /* [B, num_kv_heads, budget] */
+  int32_t* lengths_out;            /* [B] */
+  int32_t* positions_out;          /* [B, num_kv_heads, budget] */
+  int64_t batch, capacity, num_kv_heads, head_dim, budget, recent;
+  int64_t k_seq_stride, k_row_stride, k_head_stride;
+  int64_t v_seq_stride, v_row_stride, v_head_stride;
+  int64_t k_out_seq_stride, k_out_row_stride, k_out_head_stride;
+  int64_t v_out_seq_stride, v_out_row_stride, v_out_head_stride;
+} ttj_cache_evict_args;
+
+/*
+ * Per sequence and key / value head: a cache of n <= budget rows is kept whole;
+ * of a longer one the last `recent` rows and the budget - recent heaviest of
+ * the others by key_weights are kept (equal weights: the lowest row first; NaN
+ * counts as -infinity), in their order.  positions_out gives the kept rows'
+ * indices.  Output rows past the kept ones are zeros, their positions -1.
+ */
+int ttj_cache_evict(const ttj_cache_evict_args* args, ttj_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,8 @@ EXPORTED_SYMBOLS = (
     "ttj_int8_quant_rows", "ttj_int8_gemm_s32", "ttj_int8_linear_fwd",
     "ttj_int8_attn_layer_workspace_size", "ttj_int8_attn_layer_fwd",
     "ttj_layernorm_fwd", "ttj_linear_gelu_fwd", "ttj_block_workspace_size", "ttj_transformer_block_fwd",
+    "ttj_prompt_plan_entries", "ttj_prompt_plan_build", "ttj_prompt_attn_fwd",
+    "ttj_shared_prefix_attn_workspace_size", "ttj_shared_prefix_attn_fwd", "ttj_cache_evict",
 )
 
 vp = C.c_void_p
@@ -76,6 +78,49 @@ class BlockArgs(C.Structure):
     ]
 
 
+class PromptAttnArgs(C.Structure):
+    """Mirror of ``ttj_prompt_attn_args``."""
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("out", vp), ("lse", vp), ("plan", vp),
+        ("plan_entries", i64), ("status", vp),
+        ("tokens", i64), ("num_heads", i64), ("num_kv_heads", i64), ("head_dim", i64),
+        ("q_token_stride", i64), ("q_head_stride", i64), ("k_token_stride", i64),
+        ("k_head_stride", i64), ("v_token_stride", i64), ("v_head_stride", i64),
+        ("scale", C.c_float), ("dtype", ci),
+    ]
+
+
+class SharedPrefixAttnArgs(C.Structure):
+    """Mirror of ``ttj_shared_prefix_attn_args``."""
+    _fields_ = [
+        ("q", vp), ("prefix_k", vp), ("prefix_v", vp), ("k_cache", vp), ("v_cache", vp),
+        ("lengths", vp), ("key_weights", vp), ("key_weights_out", vp), ("out", vp),
+        ("workspace", vp), ("workspace_bytes", C.c_size_t), ("status", vp),
+        ("batch", i64), ("prefix_len", i64), ("capacity", i64), ("num_heads", i64),
+        ("num_kv_heads", i64), ("head_dim", i64),
+        ("q_seq_stride", i64), ("q_head_stride", i64),
+        ("prefix_k_row_stride", i64), ("prefix_k_head_stride", i64),
+        ("prefix_v_row_stride", i64), ("prefix_v_head_stride", i64),
+        ("k_seq_stride", i64), ("k_row_stride", i64), ("k_head_stride", i64),
+        ("v_seq_stride", i64), ("v_row_stride", i64), ("v_head_stride", i64),
+        ("scale", C.c_float), ("dtype", ci),
+    ]
+
+
+class CacheEvictArgs(C.Structure):
+    """Mirror of ``ttj_cache_evict_args``."""
+    _fields_ = [
+        ("k_cache", vp), ("v_cache", vp), ("key_weights", vp), ("lengths", vp),
+        ("k_out", vp), ("v_out", vp), ("weights_out", vp), ("lengths_out", vp), ("positions_out", vp),
+        ("batch", i64), ("capacity", i64), ("num_kv_heads", i64), ("head_dim", i64),
+        ("budget", i64), ("recent", i64),
+        ("k_seq_stride", i64), ("k_row_stride", i64), ("k_head_stride", i64),
+        ("v_seq_stride", i64), ("v_row_stride", i64), ("v_head_stride", i64),
+        ("k_out_seq_stride", i64), ("k_out_row_stride", i64), ("k_out_head_stride", i64),
+        ("v_out_seq_stride", i64), ("v_out_row_stride", i64), ("v_out_head_stride", i64),
+    ]
+
+
 _SIGNATURES = {
     "ttj_version": (ci, []),
     "ttj_status_string": (C.c_char_p, [ci]),
@@ -99,6 +144,12 @@ _SIGNATURES = {
     "ttj_linear_gelu_fwd": (ci, [vp, vp, vp, vp, i64, i64, i64, ci, vp, vp]),
     "ttj_block_workspace_size": (C.c_size_t, [i64, i64, i64, i64, ci]),
     "ttj_transformer_block_fwd": (ci, [C.POINTER(BlockArgs), vp]),
+    "ttj_prompt_plan_entries": (i64, [C.POINTER(i64), i64, i64, i64, i64]),
+    "ttj_prompt_plan_build": (ci, [C.POINTER(i64), i64, i64, i64, i64, C.POINTER(C.c_int32), i64]),
+    "ttj_prompt_attn_fwd": (ci, [C.POINTER(PromptAttnArgs), vp]),
+    "ttj_shared_prefix_attn_workspace_size": (C.c_size_t, [i64, i64, i64, i64, i64, i64, ci]),
+    "ttj_shared_prefix_attn_fwd": (ci, [C.POINTER(SharedPrefixAttnArgs), vp]),
+    "ttj_cache_evict": (ci, [C.POINTER(CacheEvictArgs), vp]),
 }
 
 _lock = threading.Lock()

@@ -120,6 +120,29 @@ int launch_layernorm(const void* x, const void* gamma, const void* beta, const u
                      void* y, int64_t rows, int64_t d, float eps, int dtype, cudaStream_t stream,
                      int out_dtype = -1);
 
+// Serving operators.  The extern "C" layer (serving_capi.cu) has validated the
+// arguments; the ABI's structs are the launchers' arguments.
+constexpr int64_t kMaxGroup = 128;  // query heads per key / value head: one 128-row tile holds a group
+
+// One record of a prompt plan: queries q_row .. q_row + rows - 1 of the packed
+// batch, all of the prompt whose first token is row k_row.
+struct PlanEntry {
+  int32_t q_row, rows, k_row, unused;
+};
+static_assert(sizeof(PlanEntry) == 16, "the ABI's plan records are four int32");
+
+// Positions of one work item of a plan (two 128-row query tiles up to head_dim
+// 128, one above), a 128-row tile holding 128 / group positions of a whole group.
+inline int64_t plan_positions(int64_t group, int64_t head_dim) {
+  return (head_dim <= 128 ? 2 : 1) * (128 / group);
+}
+
+int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream);
+size_t shared_prefix_attn_workspace(int64_t batch, int64_t prefix_len, int64_t capacity, int64_t num_heads,
+                                    int64_t num_kv_heads, int64_t head_dim, bool with_key_weights);
+int launch_shared_prefix_attn(const ttj_shared_prefix_attn_args& a, cudaStream_t stream);
+int launch_cache_evict(const ttj_cache_evict_args& a, cudaStream_t stream);
+
 int launch_quant_rows(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols,
                       int dtype, cudaStream_t stream);
 

@@ -8,7 +8,7 @@ any error code.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -401,3 +401,234 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     s = (amax / torch.full_like(amax, 127.0)).clamp(min=1e-8)
     q = torch.round(wf / s[:, None]).to(torch.int8)
     return q.contiguous(), s.contiguous()
+
+
+# ------------------------------------------------------- serving: prompts, caches
+
+def _strided(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, Tuple[int, ...]]:
+    """(t, element strides of all dimensions but the last): views whose rows are
+    contiguous and 16-byte aligned are read in place, anything else is copied."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (got {t.device}); there is no CPU path")
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+    if (t.stride(-1) != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s <= 0 or s % 8 for _, s in lead):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    # a dimension of one element has no stride of its own; give it a valid one
+    return t, tuple(s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def _same(ref: torch.Tensor, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != ref.dtype or t.device != ref.device:
+            raise RuntimeError(f"{name} must be {ref.dtype} on {ref.device}, got {t.dtype} on {t.device}")
+
+
+def _group(num_heads: int, num_kv_heads: int) -> int:
+    if num_kv_heads <= 0 or num_heads <= 0 or num_heads % num_kv_heads:
+        raise RuntimeError(f"num_heads ({num_heads}) must be a positive multiple of num_kv_heads ({num_kv_heads})")
+    return num_heads // num_kv_heads
+
+
+class PromptPlan:
+    """Work plan of a packed batch of prompts: built once from the prompts' lengths
+    (on the host, zero lengths allowed) and read by every layer's ``prompt_attn``.
+    The copy to the device is ordered on the stream current at construction."""
+
+    def __init__(self, seq_lens: Union[Sequence[int], torch.Tensor], num_heads: int, num_kv_heads: int,
+                 head_dim: int, device: Union[torch.device, str, int]) -> None:
+        lib = _lib.load()
+        lens = [int(n) for n in (seq_lens.tolist() if isinstance(seq_lens, torch.Tensor) else seq_lens)]
+        _group(num_heads, num_kv_heads)
+        self.seq_lens = tuple(lens)
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self.tokens = sum(lens)
+        arr = (C.c_int64 * max(1, len(lens)))(*lens)
+        n = lib.ttj_prompt_plan_entries(arr, len(lens), num_heads, num_kv_heads, head_dim)
+        if n < 0:
+            _lib.check(int(n), "ttj_prompt_plan_entries")
+        host = torch.empty(max(1, n), 4, dtype=torch.int32)
+        _lib.check(lib.ttj_prompt_plan_build(arr, len(lens), num_heads, num_kv_heads, head_dim,
+                                             C.cast(host.data_ptr(), C.POINTER(C.c_int32)), n),
+                   "ttj_prompt_plan_build")
+        self.entries = int(n)
+        self.table = host.to(device)
+
+    @property
+    def device(self) -> torch.device:
+        return self.table.device
+
+
+def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PromptPlan,
+                scale: Optional[float] = None, return_lse: bool = False,
+                out: Optional[torch.Tensor] = None):
+    """Causal attention of packed prompts: q [T,Hq,hd] and k, v [T,Hkv,hd] hold the
+    plan's prompts one after another; query head h reads key / value head
+    h // (Hq / Hkv).  Returns [T,Hq,hd], and with ``return_lse`` also the log of
+    each row's sum of exponentials, fp32 [T,Hq].  Views with strided rows (slices
+    of a packed projection) are read in place.  scale defaults to hd ** -0.5."""
+    lib = _lib.load()
+    dt = _dtype_code(q)
+    want_q = (plan.tokens, plan.num_heads, plan.head_dim)
+    want_kv = (plan.tokens, plan.num_kv_heads, plan.head_dim)
+    for t, n, want in ((q, "q", want_q), (k, "k", want_kv), (v, "v", want_kv)):
+        if tuple(t.shape) != want:
+            raise RuntimeError(f"{n} must be {list(want)} for this plan, got {list(t.shape)}")
+    _same(q, k=k, v=v)
+    q, qs = _strided(q, "q")
+    k, ks = _strided(k, "k")
+    v, vs = _strided(v, "v")
+    if plan.device != q.device:
+        raise RuntimeError(f"the plan is on {plan.device}, q on {q.device}")
+    if out is None:
+        out = torch.empty(want_q, dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != want_q or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous [T,Hq,hd] tensor of q's dtype on q's device")
+    lse = torch.empty(want_q[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    a = _lib.PromptAttnArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=_ptr(lse),
+        plan=plan.table.data_ptr(), plan_entries=plan.entries, status=status_word(q.device).data_ptr(),
+        tokens=plan.tokens, num_heads=plan.num_heads, num_kv_heads=plan.num_kv_heads, head_dim=plan.head_dim,
+        q_token_stride=qs[0], q_head_stride=qs[1], k_token_stride=ks[0], k_head_stride=ks[1],
+        v_token_stride=vs[0], v_head_stride=vs[1],
+        scale=plan.head_dim ** -0.5 if scale is None else float(scale), dtype=dt)
+    with torch.cuda.device(q.device):
+        _lib.check(lib.ttj_prompt_attn_fwd(C.byref(a), _stream(q.device)), "ttj_prompt_attn_fwd")
+    return (out, lse) if return_lse else out
+
+
+def _lengths(lengths: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
+    if tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or lengths.device != device:
+        raise RuntimeError(f"lengths must be int32 [{batch}] on {device}, got {lengths.dtype} "
+                           f"{list(lengths.shape)} on {lengths.device}")
+    return lengths.contiguous()
+
+
+def _key_weights(w: torch.Tensor, shape: Tuple[int, ...], device: torch.device) -> torch.Tensor:
+    if tuple(w.shape) != shape or w.dtype != torch.float32 or w.device != device:
+        raise RuntimeError(f"key_weights must be float32 {list(shape)} on {device}, got {w.dtype} "
+                           f"{list(w.shape)} on {w.device}")
+    return w.contiguous()
+
+
+def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                       k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                       key_weights: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """One decode step: each sequence's new token q [B,Hq,hd] attends the prefix rows
+    prefix_k / prefix_v [P,Hkv,hd] that the whole batch shares, then the first
+    ``lengths[b]`` rows of its own cache k_cache / v_cache [B,C,Hkv,hd] (P and C may
+    be zero; a sequence without any key gets zeros).  Returns [B,Hq,hd].
+
+    With ``key_weights`` (fp32 [B,Hkv,C]) it returns (out, new_key_weights): each
+    cached key's weight plus this step's probabilities of that key summed over
+    the group's heads, for ``cache_evict``; the input is not written."""
+    lib = _lib.load()
+    dt = _dtype_code(q)
+    if q.dim() != 3 or prefix_k.dim() != 3 or k_cache.dim() != 4:
+        raise RuntimeError("q must be [B,Hq,hd], prefix_k and prefix_v [P,Hkv,hd], k_cache and v_cache [B,C,Hkv,hd]")
+    B, Hq, hd = q.shape
+    P, Hkv = prefix_k.shape[:2]
+    Cap = k_cache.shape[1]
+    _group(Hq, Hkv)
+    for t, n, want in ((prefix_k, "prefix_k", (P, Hkv, hd)), (prefix_v, "prefix_v", (P, Hkv, hd)),
+                       (k_cache, "k_cache", (B, Cap, Hkv, hd)), (v_cache, "v_cache", (B, Cap, Hkv, hd))):
+        if tuple(t.shape) != want:
+            raise RuntimeError(f"{n} must be {list(want)}, got {list(t.shape)}")
+    _same(q, prefix_k=prefix_k, prefix_v=prefix_v, k_cache=k_cache, v_cache=v_cache)
+    q, qs = _strided(q, "q")
+    prefix_k, pks = _strided(prefix_k, "prefix_k")
+    prefix_v, pvs = _strided(prefix_v, "prefix_v")
+    k_cache, kcs = _strided(k_cache, "k_cache")
+    v_cache, vcs = _strided(v_cache, "v_cache")
+    lengths = _lengths(lengths, B, q.device)
+    new_weights = None
+    if key_weights is not None:
+        key_weights = _key_weights(key_weights, (B, Hkv, Cap), q.device)
+        new_weights = torch.empty_like(key_weights)
+    if out is None:
+        out = torch.empty(B, Hq, hd, dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != (B, Hq, hd) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
+    need = lib.ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, int(key_weights is not None))
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    a = _lib.SharedPrefixAttnArgs(
+        q=q.data_ptr(), prefix_k=prefix_k.data_ptr(), prefix_v=prefix_v.data_ptr(),
+        k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), lengths=lengths.data_ptr(),
+        key_weights=_ptr(key_weights), key_weights_out=_ptr(new_weights), out=out.data_ptr(),
+        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(), status=status_word(q.device).data_ptr(),
+        batch=B, prefix_len=P, capacity=Cap, num_heads=Hq, num_kv_heads=Hkv, head_dim=hd,
+        q_seq_stride=qs[0], q_head_stride=qs[1],
+        prefix_k_row_stride=pks[0], prefix_k_head_stride=pks[1],
+        prefix_v_row_stride=pvs[0], prefix_v_head_stride=pvs[1],
+        k_seq_stride=kcs[0], k_row_stride=kcs[1], k_head_stride=kcs[2],
+        v_seq_stride=vcs[0], v_row_stride=vcs[1], v_head_stride=vcs[2],
+        scale=hd ** -0.5 if scale is None else float(scale), dtype=dt)
+    with torch.cuda.device(q.device):
+        _lib.check(lib.ttj_shared_prefix_attn_fwd(C.byref(a), _stream(q.device)), "ttj_shared_prefix_attn_fwd")
+    return out if new_weights is None else (out, new_weights)
+
+
+class EvictedCache(NamedTuple):
+    """``cache_evict``'s result: the compacted cache and which rows it holds."""
+    k: torch.Tensor            # [B, budget, Hkv, hd]
+    v: torch.Tensor
+    key_weights: torch.Tensor  # fp32 [B, Hkv, budget]
+    lengths: torch.Tensor      # int32 [B]
+    positions: torch.Tensor    # int32 [B, Hkv, budget], -1 past the kept rows
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Tensor,
+                lengths: torch.Tensor, budget: int, recent: int,
+                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> EvictedCache:
+    """Cut each cache k_cache / v_cache [B,C,Hkv,hd] to ``budget`` rows per key / value
+    head: the last ``recent`` of its ``lengths[b]`` rows and, of the others, those
+    with the largest accumulated attention weight (key_weights, fp32 [B,Hkv,C];
+    equal weights: the lowest row first; NaN counts as -infinity), in their order.
+    Caches of at most ``budget`` rows are kept whole.  Rows past the kept ones are
+    zeros.  ``out`` = (k, v) of at least ``budget`` rows takes the result in place
+    of fresh caches (rows from ``budget`` on are left alone); it must not alias
+    the input."""
+    lib = _lib.load()
+    _dtype_code(k_cache)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise RuntimeError(f"k_cache and v_cache must both be [B,C,Hkv,hd], got {list(k_cache.shape)} and {list(v_cache.shape)}")
+    B, Cap, Hkv, hd = k_cache.shape
+    budget, recent = int(budget), int(recent)
+    if budget <= 0 or recent < 0 or recent > budget:
+        raise RuntimeError(f"budget must be positive and recent in 0 .. budget, got {budget} and {recent}")
+    _same(k_cache, v_cache=v_cache)
+    dev = k_cache.device
+    k_cache, kcs = _strided(k_cache, "k_cache")
+    v_cache, vcs = _strided(v_cache, "v_cache")
+    lengths = _lengths(lengths, B, dev)
+    key_weights = _key_weights(key_weights, (B, Hkv, Cap), dev)
+    if out is None:
+        k_out = torch.empty(B, budget, Hkv, hd, dtype=k_cache.dtype, device=dev)
+        v_out = torch.empty_like(k_out)
+    else:
+        k_out, v_out = out
+        _same(k_cache, k_out=k_out, v_out=v_out)
+        for t, n in ((k_out, "k_out"), (v_out, "v_out")):
+            if t.dim() != 4 or t.shape[0] != B or t.shape[1] < budget or tuple(t.shape[2:]) != (Hkv, hd):
+                raise RuntimeError(f"{n} must be [{B}, >={budget}, {Hkv}, {hd}], got {list(t.shape)}")
+    (ko, kos), (vo, vos) = _strided(k_out, "k_out"), _strided(v_out, "v_out")
+    if ko is not k_out or vo is not v_out:
+        raise RuntimeError("out must have contiguous rows and 16-byte aligned strides")
+    weights = torch.empty(B, Hkv, budget, dtype=torch.float32, device=dev)
+    new_lengths = torch.empty(B, dtype=torch.int32, device=dev)
+    positions = torch.empty(B, Hkv, budget, dtype=torch.int32, device=dev)
+    a = _lib.CacheEvictArgs(
+        k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), key_weights=key_weights.data_ptr(),
+        lengths=lengths.data_ptr(), k_out=k_out.data_ptr(), v_out=v_out.data_ptr(),
+        weights_out=weights.data_ptr(), lengths_out=new_lengths.data_ptr(), positions_out=positions.data_ptr(),
+        batch=B, capacity=Cap, num_kv_heads=Hkv, head_dim=hd, budget=budget, recent=recent,
+        k_seq_stride=kcs[0], k_row_stride=kcs[1], k_head_stride=kcs[2],
+        v_seq_stride=vcs[0], v_row_stride=vcs[1], v_head_stride=vcs[2],
+        k_out_seq_stride=kos[0], k_out_row_stride=kos[1], k_out_head_stride=kos[2],
+        v_out_seq_stride=vos[0], v_out_row_stride=vos[1], v_out_head_stride=vos[2])
+    with torch.cuda.device(dev):
+        _lib.check(lib.ttj_cache_evict(C.byref(a), _stream(dev)), "ttj_cache_evict")
+    return EvictedCache(k_out, v_out, weights, new_lengths, positions)
