@@ -6,8 +6,9 @@ import math
 import torch
 
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
-# half a unit in the last place, relative: 11 and 8 significant bits
-UNIT = {torch.float16: 2.0 ** -12, torch.bfloat16: 2.0 ** -9}
+# half a unit in the last place, relative: 11 and 8 significant bits (the value
+# halfway from 1 to its upper neighbour, 1 + 2^-11 and 1 + 2^-8, is off by that much)
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
 def attend(q, k, v, scale, visible=None):
