@@ -1,0 +1,982 @@
+// Grouped-head attention on the tensor cores: causal attention over packed
+// prompts, and attention of a batch of single tokens over a prefix they share.
+//
+//   o_r = sum_u p_ru v_u,  p_ru = 2^(c q_r.k_u - m_r) / l_r,  c = scale log2(e),
+// computed key tile by key tile with a running reference m_r and sum l_r (the
+// recurrence of an online softmax; m moves only when a tile exceeds it by 2^8).
+//
+// The group packs into the tile.  A 128-row query tile holds P = 128 / group
+// consecutive positions times the group's heads (row = position * group + head):
+// one TMA box [P][group][64 columns] of q lands as exactly these rows, K and V of
+// the one key / value head are read once for the whole group, and a prompt of 20
+// tokens with 4 heads per group fills 80 of 128 rows instead of 4 tiles of 20.
+// (group not dividing 128: the last 128 - P * group rows idle.)  For the shared
+// prefix the "positions" are the batch's sequences, so its K and V tiles are read
+// once for all of them.
+//
+// Work item = (key / value head, 2 P consecutive positions of one prompt) = query
+// tiles A and B that share every K/V tile (head_dim above 128: one tile), or, for
+// the prefix, (head, 2 P sequences, a range of the prefix's keys), whose partial
+// result (o, log2 of the sum) a later kernel joins.  One persistent CTA per SM,
+// items dealt longest first in snake order.
+//
+// Keys that no row of an item may see (later tokens, the next prompt's, rows past
+// the tensor) can sit in its last K/V tile and hold anything: their scores are
+// replaced by -inf before any arithmetic, and P.V reads V only up to the last
+// visible key rounded up to 16 rows, the rounding's rows zeroed in shared memory
+// (0 * NaN would not be 0).
+//
+// Roles, tensor-memory layouts and schedules are those of the dense kernel
+// (flash_attn_sm100.cu), whose measurements chose them:
+//   warp 0       TMA: K_j / V_j tiles into rings, item after item
+//   warps 1, 3   MMA issue (one lane): S_t = Q_t K_j^T into TMEM, O_t += P_t V_j with
+//                P read from TMEM; head_dim 64: warp 1 tile A, warp 3 tile B;
+//                above: warp 1 for both
+//   warp 2       TMA: the items' Q tiles
+//   warps 4..    softmax: head_dim 64, 8 warps per tile with 16 rows each, P in its
+//                own TMEM columns; above, 4 warps per tile with 32 rows each, P
+//                written over S
+#include <atomic>
+
+#include "attn_math.cuh"
+#include "sm100_ptx.cuh"
+#include "ttj_internal.h"
+
+namespace ttj {
+namespace {
+
+constexpr int kTile = 128;                  // rows of a query tile, keys of a K/V tile
+constexpr int kChunkBytes = 128 * 128;      // [128 rows][64 columns] of 16-bit, swizzled
+constexpr uint32_t kTmemCols = 512;
+constexpr int64_t kHeadMajorKvBytes = int64_t(96) << 20;
+
+struct GroupedParams {
+  void* out;              // prompts: [T, Hq, hd]
+  float* lse;             // prompts: [T, Hq] or null
+  const int4* plan;       // prompts: PlanEntry records
+  float* part_o;          // prefix: [splits][B][Hq][hd]
+  float* part_lse;        // prefix: [splits][B][Hq], log2 of the sum of exponentials
+  int num_items, num_entries, kv_heads, group, positions;  // positions = 128 / group
+  int num_heads, hd;
+  int head_major;         // item order: 1 = a head's entries consecutive
+  int batch, prefix, split_keys, row_items;  // prefix: row_items = ceil(B / (tiles * positions))
+  float scale_log2;
+  int* status;
+};
+
+template <int HD>
+struct GroupedSmem {
+  static_assert(HD == 64 || HD == 128 || HD == 256, "padded head sizes");
+  static constexpr int kNT = HD == 256 ? 1 : 2;
+  static constexpr bool kSepP = HD == 64;
+  static constexpr int kThreads = kSepP ? 640 : 384;
+  static constexpr int kLaunchRegs = kSepP ? 96 : 168;
+  static constexpr uint32_t kRegsCtl = kSepP ? 64 : 136;
+  static constexpr uint32_t kRegsSoftmax = kSepP ? 104 : 184;
+  static_assert(128 * kRegsCtl + (kThreads - 128) * kRegsSoftmax == kThreads * kLaunchRegs,
+                "register split must use the launch budget");
+  static constexpr int kEpiRows = kSepP ? 16 : 32;   // rows of a softmax warp's staging box
+  static constexpr int kStages = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  static constexpr int kTileBytes = HD * 2 * 128;
+  static constexpr int kQBufs = HD == 64 ? 2 : 1;
+  static constexpr int kQOff = 0;                    // [kQBufs][Q_A, Q_B]
+  static constexpr int kKOff = kNT * kQBufs * kTileBytes;
+  static constexpr int kVOff = kKOff + kStages * kTileBytes;
+  static constexpr int kEpiOff = kVOff + kStages * kTileBytes;
+  static constexpr int kBarOff = kEpiOff + (kThreads / 32 - 4) * kEpiRows * 128;
+  static constexpr int kTotal = 1024 + kBarOff + 512;
+  static_assert(kTotal <= 232448, "shared memory budget");
+  static constexpr uint32_t kColP = kSepP ? 256 : 0;    // + t*64 (separate) / + t*128 (over S)
+  static constexpr uint32_t kPStride = kSepP ? 64 : 128;
+  static constexpr uint32_t kColO = kSepP ? 384 : 256;  // + t*HD
+};
+
+// One work item: positions q0 .. q0 + nq - 1, keys k0 .. k0 + nk - 1; position
+// q0 + i sees keys up to k0 + rel + i (prompts) or all nk of them (prefix).
+struct Seg {
+  int q0, nq, k0, nk, rel, kvh, part;
+};
+
+template <bool PREFIX, int NT>
+__device__ __forceinline__ Seg seg_of(int item, const GroupedParams& p) {
+  Seg s;
+  if constexpr (PREFIX) {
+    const int per_head = p.num_entries;  // row items x splits
+    s.kvh = item / per_head;
+    const int r = item - s.kvh * per_head;
+    s.part = r / p.row_items;
+    s.q0 = (r - s.part * p.row_items) * NT * p.positions;
+    s.nq = min(NT * p.positions, p.batch - s.q0);
+    s.k0 = s.part * p.split_keys;
+    s.nk = min(p.split_keys, p.prefix - s.k0);
+    s.rel = 0;
+  } else {
+    int e;
+    if (p.head_major) {
+      s.kvh = item / p.num_entries;
+      e = item - s.kvh * p.num_entries;
+    } else {
+      e = item / p.kv_heads;
+      s.kvh = item - e * p.kv_heads;
+    }
+    const int4 w = __ldg(p.plan + e);
+    s.q0 = w.x;
+    s.nq = w.y;
+    s.k0 = w.z;
+    s.rel = w.x - w.z;
+    s.nk = s.rel + w.y;
+    s.part = 0;
+  }
+  return s;
+}
+
+// Keys that tile t's last position sees (0: the tile has no position).
+template <bool PREFIX>
+__device__ __forceinline__ int tile_keys(const Seg& s, int t, int positions) {
+  const int np = min(positions, s.nq - t * positions);
+  if (np <= 0) return 0;
+  return PREFIX ? s.nk : s.rel + t * positions + np;
+}
+__device__ __forceinline__ int key_tiles(int keys) { return (keys + kTile - 1) / kTile; }
+
+// Key tiles the item loads: a second tile that has positions sees at least as
+// many as the first.
+template <bool PREFIX, int NT>
+__device__ __forceinline__ int item_tiles(const Seg& s, int positions) {
+  const int a = key_tiles(tile_keys<PREFIX>(s, 0, positions));
+  return NT == 2 ? max(a, key_tiles(tile_keys<PREFIX>(s, 1, positions))) : a;
+}
+
+// Where row r of a tile (r = position * group + head) goes: its row index in
+// [tokens][Hq] (or [sequences][Hq]), or -1 for a row that is no position's.
+__device__ __forceinline__ int64_t row_index(int r, int t, const Seg& s, const GroupedParams& p) {
+  const int pos = r / p.group;
+  const int at = t * p.positions + pos;
+  if (pos >= p.positions || at >= s.nq) return -1;
+  return (int64_t)(s.q0 + at) * p.num_heads + s.kvh * p.group + (r - pos * p.group);
+}
+
+// Last key (relative to the item's first) that row r of tile t sees.
+template <bool PREFIX>
+__device__ __forceinline__ int row_limit(int r, int t, const Seg& s, const GroupedParams& p) {
+  return PREFIX ? s.nk - 1 : s.rel + t * p.positions + r / p.group;
+}
+
+// Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled)
+// of tile rows r0 .. to the output rows they belong to, 16 bytes per lane.
+template <typename T, int ROWS>
+__device__ __forceinline__ void store_box(uint32_t box, int r0, int t, int col0, const Seg& s, const GroupedParams& p) {
+  const int lane = threadIdx.x & 31;
+  const int col = col0 + 8 * (lane & 7);
+#pragma unroll
+  for (int i = 0; i < ROWS; i += 4) {
+    const int row = i + (lane >> 3);
+    const int64_t at = row_index(r0 + row, t, s, p);
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                 : "r"(box + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) : "memory");
+    if (at >= 0 && col < p.hd) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.hd + col) = w;
+  }
+}
+
+// Softmax, two warps per tile and TMEM lane quarter (head_dim 64): warp w serves
+// tile (w - 4) / 8 and 16 rows; lane 4g + k holds rows g and g + 8 of them and of
+// each 8-key group n keys 8n + 2k and 8n + 2k + 1 (the 16-lane TMEM shapes).
+template <typename T, int HD, bool PREFIX>
+__device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* epi_base, uint32_t tmem,
+                                              uint64_t* s_full, uint64_t* s_free, uint64_t* p_full,
+                                              uint64_t* o_done, volatile int* abort_flag) {
+  using L = GroupedSmem<HD>;
+  static_assert(HD == 64 && L::kSepP, "separate P, one 64-column output");
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int t = (warp - 4) >> 3;
+  const int g = lane >> 2, kq = lane & 3;
+  const int r0 = (warp & 3) * 32 + (((warp - 4) >> 2) & 1) * 16;  // this warp's first row of the tile
+  const uint32_t t_lane = tmem + (static_cast<uint32_t>(r0) << 16);
+  const uint32_t t_s = t_lane + t * 128;
+  const uint32_t t_p = t_lane + L::kColP + t * 64;
+  const uint32_t t_o = t_lane + L::kColO + t * HD;
+  const uint32_t box = smem_u32(epi_base) + (warp - 4) * (L::kEpiRows * 128);
+  uint32_t sf_phase = 0, od_phase = 0;
+  auto row_max4 = [](float v) {  // over the four threads of a row
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+  };
+  auto row_sum4 = [](float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+  };
+  bool ok = true;
+  for (int k = 0; ok; ++k) {
+    const int item = item_of(k);
+    if (item >= p.num_items) break;
+    int n_kv, lim_a, lim_b, lim_first;
+    {
+      const Seg s = seg_of<PREFIX, L::kNT>(item, p);
+      n_kv = key_tiles(tile_keys<PREFIX>(s, t, p.positions));
+      lim_a = row_limit<PREFIX>(r0 + g, t, s, p) - 2 * kq;
+      lim_b = row_limit<PREFIX>(r0 + g + 8, t, s, p) - 2 * kq;
+      lim_first = row_limit<PREFIX>(0, t, s, p);
+    }
+    if (n_kv == 0) continue;
+    float m_a = -INFINITY, m_b = -INFINITY;  // exponent references (log2 units), moved lazily
+    float l_a = 0.f, l_b = 0.f;              // this thread's part of each row's sum
+    for (int j = 0; j < n_kv; ++j) {
+      if (!mbar_wait_warp(&s_full[t], sf_phase, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+      sf_phase ^= 1u;
+      tc_fence_after();
+      float s[64];  // s[4n + e]: row (e < 2 ? a : b), key 8n + 2k + (e & 1)
+      {
+        uint32_t u[64];
+        tmem_ld_16x256b_x16(t_s, u);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(u[i]);
+      }
+      tc_fence_before();
+      mbar_arrive(&s_free[t]);  // the tensor core may overwrite S_t now
+      const int k0 = j * kTile;
+      if (k0 + kTile - 1 > lim_first) {
+        // key k0 + 8n + 2k + (e & 1) is visible iff 8n + (e & 1) <= limit - k0 - 2k
+        const int da = lim_a - k0, db = lim_b - k0;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          s[4 * n + 0] = 8 * n <= da ? s[4 * n + 0] : -INFINITY;
+          s[4 * n + 1] = 8 * n + 1 <= da ? s[4 * n + 1] : -INFINITY;
+          s[4 * n + 2] = 8 * n <= db ? s[4 * n + 2] : -INFINITY;
+          s[4 * n + 3] = 8 * n + 1 <= db ? s[4 * n + 3] : -INFINITY;
+        }
+      }
+      float ma[4], mb[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        ma[c] = fmaxf(s[16 * c + 0], s[16 * c + 1]);
+        mb[c] = fmaxf(s[16 * c + 2], s[16 * c + 3]);
+#pragma unroll
+        for (int n = 4 * c + 1; n < 4 * c + 4; ++n) {
+          ma[c] = fmax3(ma[c], s[4 * n], s[4 * n + 1]);
+          mb[c] = fmax3(mb[c], s[4 * n + 2], s[4 * n + 3]);
+        }
+      }
+      const float mxa = row_max4(fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3])));
+      const float mxb = row_max4(fmaxf(fmaxf(mb[0], mb[1]), fmaxf(mb[2], mb[3])));
+      const float mta = mxa * p.scale_log2, mtb = mxb * p.scale_log2;
+      const float mna = (mta > m_a + 8.f) ? mta : m_a;
+      const float mnb = (mtb > m_b + 8.f) ? mtb : m_b;
+      const float mua = mna == -INFINITY ? 0.f : mna;
+      const float mub = mnb == -INFINITY ? 0.f : mnb;
+      const float alpha_a = fast_exp2(m_a - mua);
+      const float alpha_b = fast_exp2(m_b - mub);
+      const uint64_t c2 = f2_pack(p.scale_log2, p.scale_log2);
+      const uint64_t nma = f2_pack(-mua, -mua), nmb = f2_pack(-mub, -mub);
+      uint32_t pk[32];  // P words: pk[2n] row a, pk[2n + 1] row b, word column 4n + k
+      uint64_t sa2[2] = {0ull, 0ull}, sb2[2] = {0ull, 0ull};
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        float x0, x1;
+        f2_unpack(ffma2(f2_pack(s[4 * n], s[4 * n + 1]), c2, nma), x0, x1);
+        const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+        pk[2 * n] = Pack<T>::two(e0, e1);
+        sa2[n & 1] = fadd2(sa2[n & 1], f2_pack(e0, e1));
+        f2_unpack(ffma2(f2_pack(s[4 * n + 2], s[4 * n + 3]), c2, nmb), x0, x1);
+        const float e2 = fast_exp2(x0), e3 = fast_exp2(x1);
+        pk[2 * n + 1] = Pack<T>::two(e2, e3);
+        sb2[n & 1] = fadd2(sb2[n & 1], f2_pack(e2, e3));
+      }
+      float a0, a1, b0, b1;
+      f2_unpack(fadd2(sa2[0], sa2[1]), a0, a1);
+      f2_unpack(fadd2(sb2[0], sb2[1]), b0, b1);
+      l_a = l_a * alpha_a + (a0 + a1);
+      l_b = l_b * alpha_b + (b0 + b1);
+      m_a = mna;
+      m_b = mnb;
+      if (j > 0) {
+        // P_t(j-1) V must have completed: it reads the P buffer written here and
+        // is the last write to O_t before a rescale.
+        if (!mbar_wait_warp(&o_done[t], od_phase, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+        od_phase ^= 1u;
+        tc_fence_after();
+      }
+      tmem_st_16x128b_x16(t_p, pk);
+      if (j > 0 && __any_sync(0xffffffffu, alpha_a != 1.f || alpha_b != 1.f)) {
+        uint32_t o[32];
+        tmem_ld_16x256b_x8(t_o, o);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          o[4 * n + 0] = __float_as_uint(__uint_as_float(o[4 * n + 0]) * alpha_a);
+          o[4 * n + 1] = __float_as_uint(__uint_as_float(o[4 * n + 1]) * alpha_a);
+          o[4 * n + 2] = __float_as_uint(__uint_as_float(o[4 * n + 2]) * alpha_b);
+          o[4 * n + 3] = __float_as_uint(__uint_as_float(o[4 * n + 3]) * alpha_b);
+        }
+        tmem_st_16x256b_x8(t_o, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (!ok) break;
+    l_a = row_sum4(l_a);
+    l_b = row_sum4(l_b);
+    const float inv_a = 1.f / l_a, inv_b = 1.f / l_b;
+    const Seg s = seg_of<PREFIX, L::kNT>(item, p);
+    float* lse = PREFIX ? p.part_lse + (int64_t)s.part * p.batch * p.num_heads : p.lse;
+    if (lse != nullptr && kq < 2) {  // one thread per row
+      const int64_t at = row_index(r0 + g + 8 * kq, t, s, p);
+      const float v = kq == 0 ? m_a + log2f(l_a) : m_b + log2f(l_b);
+      if (at >= 0) lse[at] = PREFIX ? v : v * 0.69314718055994531f;
+    }
+    if (!mbar_wait_warp(&o_done[t], od_phase, p.status, kDevTimeoutSoftmax, abort_flag)) break;
+    od_phase ^= 1u;
+    tc_fence_after();
+    uint32_t o[32];  // o[4n + e]: row (e < 2 ? a : b), column 8n + 2k + (e & 1)
+    tmem_ld_16x256b_x8(t_o, o);
+    if constexpr (PREFIX) {
+      const int64_t ra = row_index(r0 + g, t, s, p), rb = row_index(r0 + g + 8, t, s, p);
+      float* part = p.part_o + (int64_t)s.part * p.batch * p.num_heads * p.hd;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int col = 8 * n + 2 * kq;
+        if (col >= p.hd) break;
+        if (ra >= 0) *reinterpret_cast<float2*>(part + ra * p.hd + col) =
+            make_float2(__uint_as_float(o[4 * n]) * inv_a, __uint_as_float(o[4 * n + 1]) * inv_a);
+        if (rb >= 0) *reinterpret_cast<float2*>(part + rb * p.hd + col) =
+            make_float2(__uint_as_float(o[4 * n + 2]) * inv_b, __uint_as_float(o[4 * n + 3]) * inv_b);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        // 128-byte rows, 16-byte chunk n holds columns 8n..8n+7, swizzled by row & 7
+        const uint32_t wa = Pack<T>::two(__uint_as_float(o[4 * n]) * inv_a, __uint_as_float(o[4 * n + 1]) * inv_a);
+        const uint32_t wb = Pack<T>::two(__uint_as_float(o[4 * n + 2]) * inv_b, __uint_as_float(o[4 * n + 3]) * inv_b);
+        st_shared_u32(box + g * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wa);
+        st_shared_u32(box + (g + 8) * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wb);
+      }
+      __syncwarp();
+      store_box<T, 16>(box, r0, t, 0, s, p);
+      __syncwarp();  // the box is written again at the next item's end
+    }
+    // The next item's first P.V overwrites O_t only after this thread's next
+    // p_full arrival, which follows these TMEM loads.
+  }
+}
+
+// Softmax, one warp per tile and TMEM lane quarter, thread = row, P over S
+// (head_dim 128 and 256).
+template <typename T, int HD, bool PREFIX>
+__device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* epi_base, uint32_t tmem,
+                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
+                                             volatile int* abort_flag) {
+  using L = GroupedSmem<HD>;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int t = warp >= 8 ? 1 : 0;
+  if (t >= L::kNT) return;  // one tile per item: warps 8..11 have no work
+  const int r0 = (warp & 3) * 32;
+  const int r = r0 + lane;  // row within the tile
+  const uint32_t t_lane = tmem + (static_cast<uint32_t>(r0) << 16);
+  const uint32_t t_s = t_lane + t * 128;
+  const uint32_t t_p = t_lane + L::kColP + t * L::kPStride;
+  const uint32_t t_o = t_lane + L::kColO + t * HD;
+  const uint32_t box = smem_u32(epi_base) + (warp - 4) * (L::kEpiRows * 128);
+  uint32_t sf_phase = 0, od_phase = 0;
+  bool ok = true;
+  for (int k = 0; ok; ++k) {
+    const int item = item_of(k);
+    if (item >= p.num_items) break;
+    const Seg sg = seg_of<PREFIX, L::kNT>(item, p);
+    const int n_kv = key_tiles(tile_keys<PREFIX>(sg, t, p.positions));
+    if (n_kv == 0) continue;
+    const int limit = row_limit<PREFIX>(r, t, sg, p), lim_first = row_limit<PREFIX>(0, t, sg, p);
+    float m_run = -INFINITY;  // exponent reference (log2 units), moved lazily
+    float l_run = 0.f;        // running sum of P in fp32
+    for (int j = 0; j < n_kv; ++j) {
+      if (!mbar_wait_warp(&s_full[t], sf_phase, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+      sf_phase ^= 1u;
+      tc_fence_after();
+      float s[kTile];
+      {
+        uint32_t u[kTile];
+        tmem_ld128(t_s, u);
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) s[i] = __uint_as_float(u[i]);
+      }
+      const int k0 = j * kTile;
+      if (k0 + kTile - 1 > lim_first) {
+        const int lim = limit - k0;
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) s[i] = i <= lim ? s[i] : -INFINITY;
+      }
+      // row max: eight independent chains of 3-input max
+      float mx8[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) mx8[q] = fmax3(s[q], s[8 + q], s[16 + q]);
+#pragma unroll
+      for (int i = 24; i < kTile - 8; i += 16)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], s[i + q], s[i + 8 + q]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) mx8[q] = fmaxf(mx8[q], s[kTile - 8 + q]);
+      const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+      const float m_tile = mx * p.scale_log2;
+      const float m_new = (m_tile > m_run + 8.f) ? m_tile : m_run;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = fast_exp2(m_run - m_use);  // 1 unchanged, 0 from -inf
+      const uint64_t c2 = f2_pack(p.scale_log2, p.scale_log2);
+      const uint64_t nm2 = f2_pack(-m_use, -m_use);
+      uint32_t pk[2][32];
+      uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+      for (int c = 0; c < kTile / 32; ++c) {
+        uint32_t (&pc)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[c >> 1][(c & 1) * 16]);
+#pragma unroll
+        for (int ii = 0; ii < 16; ++ii) {
+          const int i = c * 16 + ii;
+          float x0, x1;
+          f2_unpack(ffma2(f2_pack(s[2 * i], s[2 * i + 1]), c2, nm2), x0, x1);
+          const float e0 = fast_exp2(x0);
+          const float e1 = fast_exp2(x1);
+          pc[ii] = Pack<T>::two(e0, e1);
+          sum2[i & 3] = fadd2(sum2[i & 3], f2_pack(e0, e1));
+        }
+        tmem_st16(t_p + c * 16, pc);  // over the S columns already read
+      }
+      float a0, a1;
+      f2_unpack(fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3])), a0, a1);
+      l_run = l_run * alpha + (a0 + a1);
+      m_run = m_new;
+      // S_t(j) being ready means P_t(j-1) V has completed: O_t may be rescaled
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(t_o + c * 32, o);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (!ok) break;
+    const int64_t at = row_index(r, t, sg, p);
+    float* lse = PREFIX ? p.part_lse + (int64_t)sg.part * p.batch * p.num_heads : p.lse;
+    if (lse != nullptr && at >= 0) {
+      const float v = m_run + log2f(l_run);
+      lse[at] = PREFIX ? v : v * 0.69314718055994531f;
+    }
+    if (!mbar_wait_warp(&o_done[t], od_phase, p.status, kDevTimeoutSoftmax, abort_flag)) break;
+    od_phase ^= 1u;
+    tc_fence_after();
+    const float inv_l = 1.f / l_run;
+    if constexpr (PREFIX) {
+      float* part = p.part_o + ((int64_t)sg.part * p.batch * p.num_heads + at) * p.hd;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        if (32 * c >= p.hd) break;  // uniform
+        uint32_t o[32];
+        tmem_ld32(t_o + c * 32, o);
+        if (at >= 0) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (32 * c + i < p.hd)
+              *reinterpret_cast<float4*>(part + 32 * c + i) =
+                  make_float4(__uint_as_float(o[i]) * inv_l, __uint_as_float(o[i + 1]) * inv_l,
+                              __uint_as_float(o[i + 2]) * inv_l, __uint_as_float(o[i + 3]) * inv_l);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int hh = 0; hh < HD / 64; ++hh) {
+        if (64 * hh >= p.hd) break;  // only zero padding left (uniform)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + hh * 64 + c * 32, o);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = Pack<T>::two(__uint_as_float(o[8 * q + 2 * i]) * inv_l, __uint_as_float(o[8 * q + 2 * i + 1]) * inv_l);
+            const int chunk = c * 4 + q;  // 16-byte chunk of the 128-byte row
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          }
+        }
+        __syncwarp();
+        store_box<T, 32>(box, r0, t, 64 * hh, sg, p);
+        __syncwarp();
+      }
+    }
+  }
+}
+
+template <typename T, int HD, bool PREFIX>
+__global__ void __launch_bounds__(GroupedSmem<HD>::kThreads, 1)
+grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const GroupedParams p) {
+  using L = GroupedSmem<HD>;
+  constexpr int ST = L::kStages;
+  constexpr int NT = L::kNT;
+  constexpr bool kSepP = L::kSepP;
+  constexpr int kChunks = HD / 64;
+  constexpr int kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  constexpr uint32_t kIdescPV = idesc_f16(kTile, HD, kBf16, 1);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem + L::kQOff;
+  uint8_t* sK = smem + L::kKOff;
+  uint8_t* sV = smem + L::kVOff;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* q_full = bars;              // [kQBufs][2] per tile: Q_t loaded
+  uint64_t* q_empty = q_full + 4;       // [kQBufs][2] per tile: last Q_t K^T of the item done
+  uint64_t* k_full = q_empty + 4;       // [ST]
+  uint64_t* k_empty = k_full + ST;      // [2][ST] per tile: its Q_t K^T done with the stage
+  uint64_t* v_full = k_empty + 2 * ST;  // [ST]
+  uint64_t* v_empty = v_full + ST;      // [2][ST] per tile: its P_t V done with the stage
+  uint64_t* s_full = v_empty + 2 * ST;  // [2] per tile: S_t written
+  uint64_t* s_free = s_full + 2;        // [2] per tile: S_t read by the softmax (separate P)
+  uint64_t* p_full = s_free + 2;        // [2] per tile: P_t written
+  uint64_t* o_done = p_full + 2;        // [2] per tile: one phase per completed P_t V (separate P) or item
+  uint64_t* drain = o_done + 2;         // [2] per issuer: every MMA completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  constexpr int kSoftmaxThreads = kSepP ? 256 : 128;  // per tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&k_empty[t * ST + s], 1);
+        mbar_init(&v_empty[t * ST + s], 1);
+      }
+    }
+    for (int t = 0; t < 2; ++t) {
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&q_full[b * 2 + t], 1);
+        mbar_init(&q_empty[b * 2 + t], 1);
+      }
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], kSoftmaxThreads);
+      mbar_init(&p_full[t], kSoftmaxThreads);
+      mbar_init(&o_done[t], 1);
+      mbar_init(&drain[t], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (p.positions * p.group < kTile) {
+    // rows of the Q tiles that no box ever writes: zeros, so that no stale bits
+    // make their (unused) softmax rescale at every step
+    const int first = p.positions * p.group * 128;
+    for (int c = 0; c < NT * L::kQBufs * kChunks; ++c)
+      for (int i = first + threadIdx.x * 16; i < kChunkBytes; i += L::kThreads * 16)
+        *reinterpret_cast<uint4*>(sQ + c * kChunkBytes + i) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();  // the previous kernel's writes are visible from here
+  grid_launch_dependents();
+
+  if (warp < 4) {
+    setmaxnreg_dec<L::kRegsCtl>();
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------------------ K/V producer
+      // A stage is refilled once every issuer has released its previous key tile
+      // (with P over S one warp issues both tiles' products and releases through
+      // tile B's barriers).
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      auto reclaim = [&](uint64_t* empty, int kv) -> bool {
+        const int st = kv % ST;
+        const uint32_t phase = ((kv / ST) & 1) ^ 1;  // passes on the first round
+        return (!kSepP || mbar_wait(&empty[st], phase, p.status, kDevTimeoutSmemEmpty, abort_flag)) &&
+               mbar_wait(&empty[ST + st], phase, p.status, kDevTimeoutSmemEmpty, abort_flag);
+      };
+      int kv = 0;  // running K/V tile counter across items
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int item = item_of(k);
+        if (item >= p.num_items) break;
+        const Seg s = seg_of<PREFIX, NT>(item, p);
+        const int n_kv = item_tiles<PREFIX, NT>(s, p.positions);
+        for (int j = 0; j < n_kv; ++j, ++kv) {
+          const int st = kv % ST;
+          if (!reclaim(k_empty, kv)) { ok = false; break; }
+          mbar_arrive_expect_tx(&k_full[st], L::kTileBytes);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(sK + st * L::kTileBytes + c * kChunkBytes, &tm_k, &k_full[st], 64 * c, s.kvh, s.k0 + j * kTile);
+          if (!reclaim(v_empty, kv)) { ok = false; break; }
+          mbar_arrive_expect_tx(&v_full[st], L::kTileBytes);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d(sV + st * L::kTileBytes + c * kChunkBytes, &tm_v, &v_full[st], 64 * c, s.kvh, s.k0 + j * kTile);
+        }
+      }
+    } else if (warp == 2 && lane == 0) {
+      // ------------------------------------------------------------ Q producer
+      tma_prefetch_desc(&tm_q);
+      const uint32_t bytes = (uint32_t)(p.positions * p.group) * 128u * kChunks;
+      int cnt[2] = {0, 0};  // Q_t tiles loaded so far
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int item = item_of(k);
+        if (item >= p.num_items) break;
+        const Seg s = seg_of<PREFIX, NT>(item, p);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (!ok || t * p.positions >= s.nq) continue;
+          const int qb = cnt[t] % L::kQBufs;
+          const uint32_t qph = (cnt[t] / L::kQBufs) & 1;
+          ++cnt[t];
+          ok = mbar_wait(&q_empty[qb * 2 + t], qph ^ 1u, p.status, kDevTimeoutSmemEmpty, abort_flag);
+          if (!ok) continue;
+          mbar_arrive_expect_tx(&q_full[qb * 2 + t], bytes);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_4d(sQ + (qb * NT + t) * L::kTileBytes + c * kChunkBytes, &tm_q, &q_full[qb * 2 + t], 64 * c, 0,
+                        s.kvh, s.q0 + t * p.positions);
+        }
+      }
+    } else if (warp == 1 || (kSepP && warp == 3)) {
+      // ------------------------------------------------------------ MMA issue
+      // The whole warp waits (it zeroes V rows together), lane 0 issues.
+      // S_t columns of keys past the tile's last visible one are not computed:
+      // n = keys of this tile rounded up to 16 (the softmax masks the rest).
+      auto qk = [&](int t, int st, int qb, int keys) {
+        const uint32_t n = (uint32_t)min(kTile, (keys + 15) & ~15);
+        const uint32_t idesc = idesc_f16(kTile, 0, kBf16, 0) | ((n >> 3) << 17);
+        const uint32_t q_addr = smem_u32(sQ + (qb * NT + t) * L::kTileBytes);
+        const uint32_t k_addr = smem_u32(sK + st * L::kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kChunkBytes + (kk & 3) * 32;
+          umma_f16_ss(tmem + t * 128, smem_desc_sw128(q_addr + off, 16, 1024),
+                      smem_desc_sw128(k_addr + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+        }
+      };
+      auto pv = [&](int t, int st, bool accumulate, int keys) {
+        const uint32_t v_addr = smem_u32(sV + st * L::kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk) {
+          // V is MN-major: 16 keys = 16 rows of 128 bytes; next 64-column chunk at +16 KB.
+          if (16 * kk < keys)
+            umma_f16_ts(tmem + L::kColO + t * HD, tmem + L::kColP + t * L::kPStride + kk * 8,
+                        smem_desc_sw128(v_addr + kk * 16 * 128, kChunkBytes, 1024), kIdescPV,
+                        (accumulate || kk > 0) ? 1u : 0u);
+        }
+      };
+      // V rows `valid` .. up to the next multiple of 16 of a stage become zeros:
+      // P.V reads them (with P = 0 in every row that counts).
+      auto zero_v_tail = [&](int st, int valid) {
+        if ((valid & 15) == 0) return;
+        const int rows = 16 - (valid & 15);
+        for (int i = lane; i < rows * 8 * kChunks; i += 32) {
+          const int c = i / (rows * 8), w = i - c * rows * 8;
+          *reinterpret_cast<uint4*>(sV + st * L::kTileBytes + c * kChunkBytes + valid * 128 + w * 16) =
+              make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      if constexpr (kSepP) {
+        // One issuing warp per tile; the Q.K cursor runs one key tile ahead of the
+        // P.V cursor, across items: S_t(j+1) is issued once the softmax has read
+        // S_t(j) (s_free), then O_t += P_t(j) V_j once P_t(j) is written.  Key tiles
+        // that only the other query tile uses are waited for and released too: a
+        // barrier's parity can only be followed phase by phase.
+        const int t = warp == 3 ? 1 : 0;
+        int qk_k = -1, qk_j = 0, qk_kv = 0, qk_keys = 0, qk_n = 0, qk_cnt = 0;
+        bool qk_first = true;
+        auto qk_open = [&]() -> bool {
+          const int item = item_of(++qk_k);
+          if (item >= p.num_items) return false;
+          const Seg s = seg_of<PREFIX, NT>(item, p);
+          qk_keys = tile_keys<PREFIX>(s, t, p.positions);
+          qk_n = item_tiles<PREFIX, NT>(s, p.positions);
+          qk_j = 0;
+          return true;
+        };
+        bool qk_live = qk_open();
+        uint32_t sfree_ph = 0u, pf_ph = 0u;
+        auto issue_qk = [&]() -> bool {
+          if (!qk_live) return true;
+          const int keys = qk_keys - qk_j * kTile;  // this tile's keys from here on
+          const int qb = qk_cnt % L::kQBufs;
+          if (keys > 0 && qk_j == 0 &&
+              !mbar_wait_warp(&q_full[qb * 2 + t], (qk_cnt / L::kQBufs) & 1, p.status, kDevTimeoutTmaFull, abort_flag))
+            return false;
+          if (keys > 0 && !qk_first) {
+            if (!mbar_wait_warp(&s_free[t], sfree_ph, p.status, kDevTimeoutSoftmax, abort_flag)) return false;
+            sfree_ph ^= 1u;
+          }
+          const int st = qk_kv % ST;
+          if (!mbar_wait_warp(&k_full[st], (qk_kv / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
+          ++qk_kv;
+          const bool last = keys > 0 && keys <= kTile;  // the last S_t of the item: Q_t may be replaced
+          if (keys > 0) {
+            tc_fence_after();
+            if (lane == 0) {
+              qk(t, st, qb, keys);
+              umma_commit(&s_full[t]);
+              umma_commit(&k_empty[t * ST + st]);
+              if (last) umma_commit(&q_empty[qb * 2 + t]);
+            }
+            qk_first = false;
+          } else if (lane == 0) {
+            mbar_arrive(&k_empty[t * ST + st]);
+          }
+          __syncwarp();
+          if (last) ++qk_cnt;
+          if (++qk_j == qk_n) qk_live = qk_open();
+          return true;
+        };
+        bool ok = issue_qk();
+        int kv = 0;
+        for (int k = 0; ok; ++k) {
+          const int item = item_of(k);
+          if (item >= p.num_items) break;
+          const Seg s = seg_of<PREFIX, NT>(item, p);
+          const int keys = tile_keys<PREFIX>(s, t, p.positions), nk = s.nk;
+          const int n = item_tiles<PREFIX, NT>(s, p.positions);
+          for (int j = 0; j < n; ++j, ++kv) {
+            if (!issue_qk()) { ok = false; break; }
+            const bool active = j * kTile < keys;
+            if (active) {
+              if (!mbar_wait_warp(&p_full[t], pf_ph, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+              pf_ph ^= 1u;
+            }
+            const int st = kv % ST;
+            if (!mbar_wait_warp(&v_full[st], (kv / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            if (active) {
+              // both tiles' issuers may write these zeros; a product that already
+              // reads them reads zeros either way
+              if (nk - j * kTile < kTile) zero_v_tail(st, nk - j * kTile);
+              tc_fence_after();
+              if (lane == 0) {
+                pv(t, st, j > 0, keys - j * kTile);
+                umma_commit(&o_done[t]);
+                umma_commit(&v_empty[t * ST + st]);
+              }
+            } else if (lane == 0) {
+              mbar_arrive(&v_empty[t * ST + st]);
+            }
+            __syncwarp();
+          }
+        }
+        // Nothing of this warp's may still run on the tensor core when TMEM is
+        // released (matters only after an abort).
+        if (lane == 0) {
+          umma_commit(&drain[t]);
+          mbar_wait(&drain[t], 0, p.status, kDevTimeoutSoftmax, nullptr);
+        }
+        __syncwarp();
+      } else {
+        static_assert(L::kQBufs == 1, "the single-issuer schedule uses one Q buffer per tile");
+        // P over S: one warp issues both tiles, PV_A(j) QK_A(j+1) PV_B(j) QK_B(j+1).
+        // Stages are released through tile B's barriers, once every earlier
+        // product of this thread has completed.
+        int kv = 0;
+        uint32_t pf_phase[2] = {0u, 0u}, q_phase[2] = {0u, 0u};
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+          const int item = item_of(k);
+          if (item >= p.num_items) break;
+          const Seg s = seg_of<PREFIX, NT>(item, p);
+          const int keys_a = tile_keys<PREFIX>(s, 0, p.positions);
+          const int keys_b = NT == 2 ? tile_keys<PREFIX>(s, 1, p.positions) : 0;
+          const int n_a = key_tiles(keys_a), n_b = key_tiles(keys_b), n = max(n_a, n_b);
+          const int nk = s.nk;
+          if (!mbar_wait_warp(&q_full[0], q_phase[0], p.status, kDevTimeoutTmaFull, abort_flag)) break;
+          q_phase[0] ^= 1u;
+          if (n_b > 0) {
+            if (!mbar_wait_warp(&q_full[1], q_phase[1], p.status, kDevTimeoutTmaFull, abort_flag)) break;
+            q_phase[1] ^= 1u;
+          }
+          const int kv0 = kv;
+          {
+            const int st = kv0 % ST;
+            if (!mbar_wait_warp(&k_full[st], (kv0 / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) break;
+            tc_fence_after();
+            if (lane == 0) {
+              qk(0, st, 0, keys_a);
+              umma_commit(&s_full[0]);
+              if (n_a == 1) umma_commit(&q_empty[0]);
+              if (n_b > 0) {
+                qk(1, st, 0, keys_b);
+                umma_commit(&s_full[1]);
+                if (n_b == 1) umma_commit(&q_empty[1]);
+              }
+              umma_commit(&k_empty[ST + st]);
+            }
+            __syncwarp();
+          }
+          for (int j = 0; j < n; ++j) {
+            const int st = (kv0 + j) % ST;
+            const int st_n = (kv0 + j + 1) % ST;
+            const int left = nk - j * kTile;  // keys of the item from this tile on
+            if (j + 1 < n && !mbar_wait_warp(&k_full[st_n], ((kv0 + j + 1) / ST) & 1, p.status, kDevTimeoutTmaFull,
+                                             abort_flag)) { ok = false; break; }
+            if (!mbar_wait_warp(&v_full[st], ((kv0 + j) / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            if (left < kTile) zero_v_tail(st, left);
+            if (j < n_a) {
+              if (!mbar_wait_warp(&p_full[0], pf_phase[0], p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+              pf_phase[0] ^= 1u;
+              tc_fence_after();
+              if (lane == 0) {
+                pv(0, st, j > 0, keys_a - j * kTile);
+                if (j + 1 < n_a) {
+                  qk(0, st_n, 0, keys_a - (j + 1) * kTile);
+                  umma_commit(&s_full[0]);
+                  if (j + 2 == n_a) umma_commit(&q_empty[0]);
+                } else {
+                  umma_commit(&o_done[0]);
+                }
+              }
+              __syncwarp();
+            }
+            if (j < n_b) {
+              if (!mbar_wait_warp(&p_full[1], pf_phase[1], p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+              pf_phase[1] ^= 1u;
+              tc_fence_after();
+            }
+            if (lane == 0) {
+              if (j < n_b) pv(1, st, j > 0, keys_b - j * kTile);
+              umma_commit(&v_empty[ST + st]);
+              if (j + 1 < n_b) {
+                qk(1, st_n, 0, keys_b - (j + 1) * kTile);
+                umma_commit(&s_full[1]);
+                if (j + 2 == n_b) umma_commit(&q_empty[1]);
+              } else if (j < n_b) {
+                umma_commit(&o_done[1]);
+              }
+              if (j + 1 < n) umma_commit(&k_empty[ST + st_n]);
+            }
+            __syncwarp();
+          }
+          kv = kv0 + n;
+        }
+        if (lane == 0) {
+          umma_commit(&drain[0]);
+          mbar_wait(&drain[0], 0, p.status, kDevTimeoutSoftmax, nullptr);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    setmaxnreg_inc<L::kRegsSoftmax>();
+    if constexpr (kSepP)
+      softmax_pairs<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, s_full, s_free, p_full, o_done, abort_flag);
+    else
+      softmax_rows<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, s_full, p_full, o_done, abort_flag);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Check the register count the kernel's setmaxnreg split assumes (with another
+// the softmax warps' increase could never complete) and opt in to its shared
+// memory, once per kernel and device.
+template <typename Kernel>
+int prepare_kernel(Kernel kern, int launch_regs, int smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  TTJ_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return TTJ_OK;
+  cudaFuncAttributes fa;
+  TTJ_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
+  if (fa.numRegs != launch_regs)
+    return fail(TTJ_ERR_UNSUPPORTED, "attention kernel register count differs from its register split");
+  TTJ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  done.fetch_or(bit, std::memory_order_release);
+  return TTJ_OK;
+}
+
+struct GroupedTensors {
+  const void *q, *k, *v;
+  int64_t q_rows, kv_rows;                  // tokens or sequences; tokens or prefix rows
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+};
+
+template <typename T, int HD, bool PREFIX>
+int launch_grouped(const GroupedTensors& x, const GroupedParams& p, cudaStream_t stream) {
+  using L = GroupedSmem<HD>;
+  const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t hd = (uint64_t)p.hd, g = (uint64_t)p.group, hkv = (uint64_t)p.kv_heads;
+  CUtensorMap tm_q, tm_k, tm_v;
+  {
+    const uint64_t dims[4] = {hd, g, hkv, (uint64_t)x.q_rows};
+    const uint64_t strides[3] = {(uint64_t)x.q_head_stride * 2, (uint64_t)x.q_head_stride * 2 * g,
+                                 (uint64_t)x.q_row_stride * 2};
+    const uint32_t box[4] = {64, (uint32_t)p.group, 1, (uint32_t)p.positions};
+    if (int rc = encode_tmap(&tm_q, dt, 4, x.q, dims, strides, box)) return rc;
+  }
+  const uint64_t dims[3] = {hd, hkv, (uint64_t)x.kv_rows};
+  const uint32_t box[3] = {64, 1, kTile};
+  const uint64_t ks[2] = {(uint64_t)x.k_head_stride * 2, (uint64_t)x.k_row_stride * 2};
+  const uint64_t vs[2] = {(uint64_t)x.v_head_stride * 2, (uint64_t)x.v_row_stride * 2};
+  if (int rc = encode_tmap(&tm_k, dt, 3, x.k, dims, ks, box)) return rc;
+  if (int rc = encode_tmap(&tm_v, dt, 3, x.v, dims, vs, box)) return rc;
+  auto kern = grouped_attn_kernel<T, HD, PREFIX>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = prepare_kernel(kern, L::kLaunchRegs, L::kTotal, done)) return rc;
+  const int grid = p.num_items < sm_count() ? p.num_items : sm_count();
+  TTJ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(L::kThreads), L::kTotal, stream, tm_q, tm_k, tm_v, p));
+  return TTJ_OK;
+}
+
+template <bool PREFIX>
+int dispatch(int dtype, const GroupedTensors& x, const GroupedParams& p, cudaStream_t stream) {
+  if (dtype == TTJ_F16) {
+    if (p.hd <= 64) return launch_grouped<__half, 64, PREFIX>(x, p, stream);
+    if (p.hd <= 128) return launch_grouped<__half, 128, PREFIX>(x, p, stream);
+    return launch_grouped<__half, 256, PREFIX>(x, p, stream);
+  }
+  if (p.hd <= 64) return launch_grouped<__nv_bfloat16, 64, PREFIX>(x, p, stream);
+  if (p.hd <= 128) return launch_grouped<__nv_bfloat16, 128, PREFIX>(x, p, stream);
+  return launch_grouped<__nv_bfloat16, 256, PREFIX>(x, p, stream);
+}
+
+}  // namespace
+
+int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
+  GroupedTensors x{a.q, a.k, a.v, a.tokens, a.tokens, a.q_token_stride, a.q_head_stride,
+                   a.k_token_stride, a.k_head_stride, a.v_token_stride, a.v_head_stride};
+  GroupedParams p{};
+  p.out = a.out;
+  p.lse = a.lse;
+  p.plan = reinterpret_cast<const int4*>(a.plan);
+  p.num_entries = (int)a.plan_entries;
+  p.kv_heads = (int)a.num_kv_heads;
+  p.num_items = (int)(a.plan_entries * a.num_kv_heads);
+  p.num_heads = (int)a.num_heads;
+  p.group = (int)(a.num_heads / a.num_kv_heads);
+  p.positions = kTile / p.group;
+  p.hd = (int)a.head_dim;
+  // As in the dense kernel: when all heads' K and V exceed about 3/4 of the L2,
+  // a head's items run consecutively and share its K/V there.
+  p.head_major = a.tokens * a.num_kv_heads * a.head_dim * 4 > kHeadMajorKvBytes ? 1 : 0;
+  p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  p.status = a.status;
+  return dispatch<false>(a.dtype, x, p, stream);
+}
+
+}  // namespace ttj

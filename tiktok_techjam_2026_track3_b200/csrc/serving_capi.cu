@@ -117,7 +117,7 @@ int ttj_prompt_attn_fwd(const ttj_prompt_attn_args* a, ttj_stream_t stream) {
   TTJ_CHECK_ARG((a->tokens == 0) == (a->plan_entries == 0) && a->plan_entries <= a->tokens, TTJ_ERR_INVALID_ARG,
                 "the plan does not belong to this many tokens");
   if (a->tokens == 0) return TTJ_OK;
-  TTJ_CHECK_ARG(a->plan_entries < ((int64_t)1 << 31) / a->num_kv_heads, TTJ_ERR_UNSUPPORTED,
+  TTJ_CHECK_ARG(a->plan_entries < (((int64_t)1 << 31) - 65536) / a->num_kv_heads, TTJ_ERR_UNSUPPORTED,
                 "too many attention work items");
   TTJ_CHECK_ARG(a->q && a->k && a->v && a->out && a->plan, TTJ_ERR_INVALID_ARG,
                 "q, k, v, out and plan must be non-NULL");
