@@ -979,4 +979,30 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
   return dispatch<false>(a.dtype, x, p, stream);
 }
 
+int launch_prefix_parts(const ttj_shared_prefix_attn_args& a, float* part_o, float* part_lse, int parts,
+                        int part_keys, cudaStream_t stream) {
+  GroupedTensors x{a.q, a.prefix_k, a.prefix_v, a.batch, a.prefix_len, a.q_seq_stride, a.q_head_stride,
+                   a.prefix_k_row_stride, a.prefix_k_head_stride, a.prefix_v_row_stride, a.prefix_v_head_stride};
+  GroupedParams p{};
+  p.part_o = part_o;
+  p.part_lse = part_lse;
+  p.kv_heads = (int)a.num_kv_heads;
+  p.num_heads = (int)a.num_heads;
+  p.group = (int)(a.num_heads / a.num_kv_heads);
+  p.positions = kTile / p.group;
+  p.hd = (int)a.head_dim;
+  p.batch = (int)a.batch;
+  p.prefix = (int)a.prefix_len;
+  p.split_keys = part_keys;
+  const int64_t per_item = plan_positions(p.group, a.head_dim);
+  p.row_items = (int)((a.batch + per_item - 1) / per_item);
+  const int64_t items = (int64_t)p.row_items * parts * a.num_kv_heads;
+  if (items >= ((int64_t)1 << 31) - 65536) return fail(TTJ_ERR_UNSUPPORTED, "too many attention work items");
+  p.num_entries = p.row_items * parts;
+  p.num_items = (int)items;
+  p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  p.status = a.status;
+  return dispatch<true>(a.dtype, x, p, stream);
+}
+
 }  // namespace ttj

@@ -551,7 +551,8 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
         out = torch.empty(B, Hq, hd, dtype=q.dtype, device=q.device)
     elif tuple(out.shape) != (B, Hq, hd) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
-    need = lib.ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, int(key_weights is not None))
+    with torch.cuda.device(q.device):
+        need = lib.ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, int(key_weights is not None))
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     a = _lib.SharedPrefixAttnArgs(
