@@ -7,6 +7,7 @@ the library is missing or fails to load, every op raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 from typing import Optional
@@ -121,6 +122,31 @@ class CacheEvictArgs(C.Structure):
     ]
 
 
+_FORMATS = {vp: "P", i64: "q", ci: "i", C.c_float: "f", C.c_size_t: "N"}
+
+
+class PackedCall:
+    """An entry point ``int f(const args*, stream)`` called with its struct's fields
+    as positional values: one ``struct`` packing instead of a ctypes assignment per
+    field (about 5 us less for 30 fields).  NULL pointers are 0."""
+
+    def __init__(self, name: str, args: type) -> None:
+        self.name = name
+        # native alignment as in C; "0P" pads the end as the compiler does
+        self._pack = struct.Struct("@" + "".join(_FORMATS[t] for _, t in args._fields_) + "0P").pack
+        self._fn = None
+
+    def __call__(self, stream: int, *values) -> None:
+        fn = self._fn
+        if fn is None:
+            fn = load()[self.name]  # a function object of its own, with its own argument types
+            fn.restype, fn.argtypes = ci, [C.c_char_p, vp]
+            self._fn = fn
+        rc = fn(self._pack(*values), stream)
+        if rc != 0:
+            check(rc, self.name)
+
+
 _SIGNATURES = {
     "ttj_version": (ci, []),
     "ttj_status_string": (C.c_char_p, [ci]),
@@ -151,6 +177,10 @@ _SIGNATURES = {
     "ttj_shared_prefix_attn_fwd": (ci, [C.POINTER(SharedPrefixAttnArgs), vp]),
     "ttj_cache_evict": (ci, [C.POINTER(CacheEvictArgs), vp]),
 }
+
+prompt_attn_fwd = PackedCall("ttj_prompt_attn_fwd", PromptAttnArgs)
+shared_prefix_attn_fwd = PackedCall("ttj_shared_prefix_attn_fwd", SharedPrefixAttnArgs)
+cache_evict = PackedCall("ttj_cache_evict", CacheEvictArgs)
 
 _lock = threading.Lock()
 _lib: Optional[C.CDLL] = None

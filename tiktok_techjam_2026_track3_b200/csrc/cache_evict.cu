@@ -1,15 +1,20 @@
 // Eviction from per-sequence caches by accumulated attention weight, two kernels.
 //
 // 1. Choosing (weights read once, 4 bytes a row): one cluster of blocks per
-//    (sequence, key / value head).  A weight compares as a 32-bit unsigned key in the
-//    order of its value; each block keeps its slice of the keys in shared memory.  The
-//    key of the last row to keep (the need-th largest) comes digit by digit, 11 + 11 +
-//    10 bits: a histogram of the digit over the keys that agree so far, summed over
-//    the cluster, tells the digit's value and how many of the rows are still to find.
-//    With `cut` that key and `ties` the rows equal to it that stay, row i's slot is
+//    (sequence, key / value head), each warp a stretch of consecutive rows.  A weight
+//    compares as a 32-bit unsigned key in the order of its value, held in registers.
+//    The key `cut` of the last row to keep (the need-th largest) is bisected two
+//    bits at a time: every warp counts its keys at or above the three candidates and
+//    the counts are summed over the cluster (one barrier).  Once at most kList keys
+//    remain between cut and its next candidate, those alone are collected (in any
+//    order: only their values count) and every block bisects on from a copy.  The
+//    search ends as soon as a candidate has exactly `need` keys.  With `ties` the rows
+//    equal to the cut that stay, row i's slot is
 //        above(i) + min(ties, equal(i)),
-//    above / equal counting the earlier rows with a larger / an equal key: both counts
-//    come from one scan, and equal rows are kept lowest index first by construction.
+//    above / equal counting the earlier rows with a larger / an equal key: equal rows
+//    are kept lowest index first by construction.
+//    (Digit histograms in shared memory took 33 us for 512 caches of 4096 rows and
+//    81 us for 32 of 65537 where this takes CHOOSE_BATCH and CHOOSE_LONG.)
 // 2. Copying (bound by the kept rows' bytes): a warp takes 32 output rows in the
 //    order of the output's memory and copies K and V rows in 16-byte pieces, eight
 //    rows in flight.
@@ -28,10 +33,11 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarpsPerBlock = kThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kSliceKeys = 8192;         // keys per block that a cluster is sized for
 constexpr int kMaxCluster = 8;
-constexpr int kMaxStagedKeys = 49152;    // 192 KB; longer slices are re-read from memory
+constexpr int kBlockKeys = 4096;         // rows per block that a cluster is sized for
+constexpr int kMaxKeysPerThread = 20;    // held in registers; longer slices are re-read
+constexpr int kList = 2 * kThreads;      // keys that the search ends on
+static_assert(32 * kMaxKeysPerThread < 1024, "a warp's three counts share one word");
 
 struct ChooseParams {
   const float* weights;   // [B][H][C]
@@ -40,8 +46,7 @@ struct ChooseParams {
   int32_t* lengths_out;
   int32_t* positions;     // [B][H][N]
   int kv_heads, capacity, budget, recent;
-  int slice;              // rows per block of the cluster (a multiple of kThreads)
-  int staged;             // the slice's keys fit in shared memory
+  int per;                // rows per thread
 };
 
 // Ascending unsigned order of the weights; NaN as -infinity, -0 as +0.
@@ -51,44 +56,43 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// A thread's keys are consecutive; one word of padding per 32 keeps them off each
-// other's banks for the row counts that occur (1 to 16 and odd ones).
-__device__ __forceinline__ int padded(int i) { return i + (i >> 5); }
-
-// Exclusive prefix over the block of two counts packed as (hi, lo) 32-bit halves,
-// and the block's total.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* warp_sums, uint64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t inc = v;
+__device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += x;
-  }
-  __syncthreads();  // the previous scan's sums have been read
-  if (lane == 31) warp_sums[warp] = inc;
-  __syncthreads();
-  uint64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarpsPerBlock; ++w) {
-    if (w < warp) before += warp_sums[w];
-    all += warp_sums[w];
-  }
-  total = all;
-  return before + inc - v;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-__global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseParams p) {
-  extern __shared__ uint32_t s_keys[];
-  __shared__ uint32_t s_hist[kBins];
-  __shared__ uint64_t s_warp[kWarpsPerBlock];
-  __shared__ uint64_t s_totals;           // this block's (above, equal), read by the cluster
-  __shared__ int s_digit, s_need;
+// State of the bisection: `need` keys are to be kept, `at` keys are >= cut, `above`
+// of them >= cut + 2^bits.
+struct Cut {
+  uint32_t cut;
+  int bits, at, above;
+  __device__ __forceinline__ uint32_t candidate(int q) const { return cut | ((uint32_t)q << (bits - 2)); }
+  __device__ __forceinline__ void take(int n1, int n2, int n3, int need) {
+    const int n[3] = {n1, n2, n3};
+    int q = n3 >= need ? 3 : (n2 >= need ? 2 : (n1 >= need ? 1 : 0));
+    if (q < 3) above = n[q];
+    if (q > 0) at = n[q - 1];
+    cut = candidate(q);
+    bits -= 2;
+  }
+};
+
+// KPT: upper bound on rows per thread, held in registers; 0: any number, read from
+// memory each time.
+template <int KPT>
+__global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) choose_kernel(const ChooseParams p) {
+  // Every warp of the cluster leaves its counts with every block: [parity][block, warp].
+  __shared__ uint32_t s_count[2][3][kMaxCluster * kWarpsPerBlock];
+  __shared__ uint64_t s_total[kMaxCluster * kWarpsPerBlock];
+  __shared__ uint32_t s_list[kList];
+  __shared__ int s_listed;
   cg::cluster_group cluster = cg::this_cluster();
   grid_dependency_wait();
   grid_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), nblocks = (int)cluster.num_blocks();
+  const int nwarps = nblocks * kWarpsPerBlock, my_warp = rank * kWarpsPerBlock + warp;
   const int64_t bh = blockIdx.x / nblocks;
   const int64_t b = bh / p.kv_heads;
   const int n = min(max(__ldg(p.lengths + b), 0), p.capacity);
@@ -96,7 +100,6 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseParams p) 
   const float* w = p.weights + bh * p.capacity;
   float* w_out = p.weights_out + bh * p.budget;
   int32_t* pos = p.positions + bh * p.budget;
-  const int first = min(rank * p.slice, n), last = min(first + p.slice, n);  // this block's rows
   if (rank == 0 && tid == 0 && bh - b * p.kv_heads == 0) p.lengths_out[b] = kept;
   // output rows past the kept ones
   for (int i = kept + rank * kThreads + tid; i < p.budget; i += nblocks * kThreads) {
@@ -104,113 +107,152 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const ChooseParams p) 
     pos[i] = -1;
   }
   if (n <= p.budget) {  // uniform over the cluster
-    for (int i = first + tid; i < last; i += kThreads) {
+    for (int i = rank * kThreads + tid; i < n; i += nblocks * kThreads) {
       w_out[i] = w[i];
       pos[i] = i;
     }
     return;
   }
-  const int old = n - p.recent;         // rows below `old` compete
-  int need = p.budget - p.recent;       // for this many places
-  const int mine = min(last, old);      // end of this block's competing rows
-  if (p.staged) {
-    for (int i = first + tid; i < last; i += kThreads) s_keys[padded(i - first)] = weight_key(w[i]);
-    __syncthreads();
+  const int old = n - p.recent;              // rows below `old` compete
+  const int need = p.budget - p.recent;      // for this many places
+  const int64_t first = (int64_t)my_warp * 32 * p.per + lane;  // rows first + 32 j
+  uint32_t key[KPT > 0 ? KPT : 1];           // 0: a row that does not compete
+  auto key_of = [&](int j) -> uint32_t {
+    const int64_t i = first + 32 * j;
+    return i < old ? weight_key(__ldg(w + i)) : 0u;
+  };
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) key[j] = j < p.per ? key_of(j) : 0u;
   }
-  auto key_at = [&](int i) -> uint32_t { return p.staged ? s_keys[padded(i - first)] : weight_key(__ldg(w + i)); };
+  // f(j, key) for this thread's rows, in order
+  auto each = [&](auto&& f) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j)
+        if (j < p.per) f(j, key[j]);
+    } else {
+      for (int j = 0; j < p.per; ++j) f(j, key_of(j));
+    }
+  };
+  if (tid == 0) s_listed = 0;
+  auto sync_all = [&]() {
+    if (nblocks > 1) cluster.sync();
+    else __syncthreads();
+  };
+  sync_all();                                // every block runs: its shared memory may be written
 
-  uint32_t cut = 0xffffffffu;           // need == 0: nothing competes
+  uint32_t cut = 0xffffffffu;                // need == 0: nothing competes
+  int ties = 0;
   if (need > 0) {
-    uint32_t prefix = 0, mask = 0;      // digits found so far
+    Cut x{0u, 32, old, 0};
+    int parity = 0;
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-      const int bins = pass == 2 ? 1024 : 2048;
-      for (int i = tid; i < kBins; i += kThreads) s_hist[i] = 0u;
-      __syncthreads();
-      for (int i0 = first; i0 < mine; i0 += kThreads) {
-        const int i = i0 + tid;
-        const uint32_t key = i < mine ? key_at(i) : 0u;
-        const bool in = i < mine && (key & mask) == prefix;
-        const uint32_t bin = in ? (key >> shift) & (bins - 1) : kBins;
-        // equal weights fall into one bin: a warp of one bin adds once
-        int same;
-        __match_all_sync(0xffffffffu, bin, &same);
-        if (same) {
-          if (in && lane == 0) atomicAdd(&s_hist[bin], 32u);
-        } else if (in) {
-          atomicAdd(&s_hist[bin], 1u);
+    do {
+      const uint32_t t1 = x.candidate(1), t2 = x.candidate(2), t3 = x.candidate(3);
+      uint32_t c1 = 0, c2 = 0, c3 = 0;
+      if constexpr (KPT > 0) {               // (keys of 0 are below every candidate)
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          c1 += key[j] >= t1;
+          c2 += key[j] >= t2;
+          c3 += key[j] >= t3;
+        }
+        // a warp's three counts share one word
+        c1 = __reduce_add_sync(0xffffffffu, c1 | c2 << 10 | c3 << 20);
+        if (lane < nblocks) *cluster.map_shared_rank(&s_count[parity][0][my_warp], lane) = c1;
+      } else {
+        each([&](int, uint32_t k) {
+          c1 += k >= t1;
+          c2 += k >= t2;
+          c3 += k >= t3;
+        });
+        c1 = __reduce_add_sync(0xffffffffu, c1);
+        c2 = __reduce_add_sync(0xffffffffu, c2);
+        c3 = __reduce_add_sync(0xffffffffu, c3);
+        if (lane < nblocks) {
+          *cluster.map_shared_rank(&s_count[parity][0][my_warp], lane) = c1;
+          *cluster.map_shared_rank(&s_count[parity][1][my_warp], lane) = c2;
+          *cluster.map_shared_rank(&s_count[parity][2][my_warp], lane) = c3;
         }
       }
-      cluster.sync();
-      // largest digit with at least `need` keys at or above it: thread t sums bins
-      // [top - 4t - 3, top - 4t] of the cluster, from the largest down
-      uint32_t c[4];
-      uint64_t sum = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int bin = bins - 1 - (4 * tid + q);
-        c[q] = 0u;
-        if (bin >= 0)
-          for (int r = 0; r < nblocks; ++r) c[q] += *cluster.map_shared_rank(&s_hist[bin], r);
-        sum += c[q];
+      sync_all();
+      c1 = c2 = c3 = 0;
+      for (int i = lane; i < nwarps; i += 32) {
+        const uint32_t v = s_count[parity][0][i];
+        c1 += KPT > 0 ? v & 1023u : v;
+        c2 += KPT > 0 ? (v >> 10) & 1023u : s_count[parity][1][i];
+        c3 += KPT > 0 ? v >> 20 : s_count[parity][2][i];
       }
-      uint64_t total;
-      uint64_t before = block_scan(sum, s_warp, total);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (before < (uint64_t)need && before + c[q] >= (uint64_t)need) {
-          s_digit = bins - 1 - (4 * tid + q);
-          s_need = need - (int)before;
+      x.take((int)__reduce_add_sync(0xffffffffu, c1), (int)__reduce_add_sync(0xffffffffu, c2),
+             (int)__reduce_add_sync(0xffffffffu, c3), need);
+      parity ^= 1;
+    } while (x.bits > 0 && x.at != need && x.at - x.above > kList);
+    if (x.bits > 0 && x.at != need) {
+      // the keys in [cut, cut + 2^bits), collected by the first block
+      uint32_t* list = cluster.map_shared_rank(s_list, 0);
+      int* listed = cluster.map_shared_rank(&s_listed, 0);
+      each([&](int, uint32_t k) {
+        const bool in = k != 0u && (k ^ x.cut) >> x.bits == 0u;  // bits <= 30 here
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (who != 0u) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(listed, __popc(who));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+          if (in) list[at] = k;
         }
-        before += c[q];
-      }
-      cluster.sync();  // the digit is known, every block has read the histograms
-      prefix |= (uint32_t)s_digit << shift;
-      mask |= (uint32_t)(bins - 1) << shift;
-      need = s_need;
+      });
+      sync_all();
+      const int count = x.at - x.above;
+      const uint32_t k0 = tid < count ? list[tid] : 0u, k1 = tid + kThreads < count ? list[tid + kThreads] : 0u;
+      const int outside = x.above;           // keys above every listed one
+#pragma unroll 1
+      do {
+        const uint32_t t1 = x.candidate(1), t2 = x.candidate(2), t3 = x.candidate(3);
+        uint32_t c = ((k0 >= t1) + (k1 >= t1)) | ((k0 >= t2) + (k1 >= t2)) << 10 | ((k0 >= t3) + (k1 >= t3)) << 20;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (lane == 0) s_count[parity][0][warp] = c;
+        __syncthreads();
+        c = lane < kWarpsPerBlock ? s_count[parity][0][lane] : 0u;
+        // at most 64 keys a warp, 1024 a block: two counts to a word
+        const uint32_t lo = __reduce_add_sync(0xffffffffu, (c & 1023u) | ((c >> 10) & 1023u) << 16);
+        const uint32_t hi = __reduce_add_sync(0xffffffffu, c >> 20);
+        x.take(outside + (int)(lo & 0xffffu), outside + (int)(lo >> 16), outside + (int)hi, need);
+        parity ^= 1;
+      } while (x.bits > 0 && x.at != need);
     }
-    cut = prefix;
+    if (x.at == need) cut = x.cut - 1u;      // exactly the keys >= cut stay (cut > 0: old > need)
+    else cut = x.cut, ties = need - x.above; // every bit found: rows equal to the cut fill up
   }
-  const int ties = need;                // of the rows equal to `cut`, the first `ties` stay
 
-  // counts over this thread's consecutive rows, then over the block, then the cluster
-  const int per = p.slice / kThreads;
-  const int from = min(first + tid * per, last), to = min(from + per, last);
-  uint32_t above = 0, equal = 0;
-  for (int i = from; i < to; ++i) {
-    if (i >= old) {
-      ++above;
-    } else {
-      const uint32_t key = key_at(i);
-      above += key > cut;
-      equal += key == cut;
-    }
-  }
-  uint64_t total;
-  uint64_t before = block_scan((uint64_t)above << 32 | equal, s_warp, total);
-  if (tid == 0) s_totals = total;
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_totals, r);
-  uint32_t a = (uint32_t)(before >> 32), e = (uint32_t)before;
-  for (int i = from; i < to; ++i) {
-    bool keep;
-    const uint32_t slot = a + min((uint32_t)ties, e);
-    if (i >= old) {
-      keep = true;
-      ++a;
-    } else {
-      const uint32_t key = key_at(i);
-      keep = key > cut || (key == cut && e < (uint32_t)ties);
-      a += key > cut;
-      e += key == cut;
-    }
-    if (keep) {
-      pos[slot] = i;
+  // This warp's rows above and equal to the cut, then those of the warps before it.
+  uint32_t a = 0, e = 0;
+  each([&](int j, uint32_t k) {
+    const int64_t i = first + 32 * j;
+    a += __popc(__ballot_sync(0xffffffffu, i < old ? k > cut : i < n));
+    e += __popc(__ballot_sync(0xffffffffu, i < old && k == cut));
+  });
+  if (lane < nblocks) *cluster.map_shared_rank(&s_total[my_warp], lane) = (uint64_t)a << 32 | e;
+  sync_all();                                // (also: no block leaves while its list is read)
+  uint64_t before = 0;
+  for (int i = lane; i < my_warp; i += 32) before += s_total[i];
+  before = warp_sum(before);
+  a = (uint32_t)(before >> 32);
+  e = (uint32_t)before;
+  const uint32_t lower = (1u << lane) - 1u;
+  each([&](int j, uint32_t k) {
+    const int64_t i = first + 32 * j;
+    const bool above = i < old ? k > cut : i < n, equal = i < old && k == cut;
+    const uint32_t ab = __ballot_sync(0xffffffffu, above), eb = __ballot_sync(0xffffffffu, equal);
+    const uint32_t e_before = e + __popc(eb & lower);
+    if (above || (equal && e_before < (uint32_t)ties)) {
+      const uint32_t slot = a + __popc(ab & lower) + min((uint32_t)ties, e_before);
+      pos[slot] = (int32_t)i;
       w_out[slot] = __ldg(w + i);
     }
-  }
-  cluster.sync();  // no block leaves while another reads its shared memory
+    a += __popc(ab);
+    e += __popc(eb);
+  });
 }
 
 struct CopyParams {
@@ -288,20 +330,11 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyParams p) {
   }
 }
 
-int launch_choose(const ChooseParams& p, int64_t caches, int cluster, int smem, cudaStream_t stream) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  TTJ_CUDA_TRY(cudaGetDevice(&dev));
-  const uint64_t bit = (uint64_t)1 << (dev & 63);
-  if (dev >= 64 || !(done.load(std::memory_order_acquire) & bit)) {
-    TTJ_CUDA_TRY(cudaFuncSetAttribute(choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (kMaxStagedKeys + kMaxStagedKeys / 32) * 4));
-    done.fetch_or(bit, std::memory_order_release);
-  }
+template <int KPT>
+int launch_choose(const ChooseParams& p, int64_t caches, int cluster, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(caches * cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -312,7 +345,7 @@ int launch_choose(const ChooseParams& p, int64_t caches, int cluster, int smem, 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  TTJ_CUDA_TRY(cudaLaunchKernelEx(&cfg, choose_kernel, p));
+  TTJ_CUDA_TRY(cudaLaunchKernelEx(&cfg, choose_kernel<KPT>, p));
   return TTJ_OK;
 }
 
@@ -331,13 +364,15 @@ int launch_cache_evict(const ttj_cache_evict_args& a, cudaStream_t stream) {
   c.budget = (int)a.budget;
   c.recent = (int)a.recent;
   int cluster = 1;
-  while (cluster < kMaxCluster && (int64_t)cluster * kSliceKeys < a.capacity) cluster *= 2;
+  while (cluster < kMaxCluster && (int64_t)cluster * kBlockKeys < a.capacity) cluster *= 2;
   if (caches * cluster >= (int64_t)1 << 31) return fail(TTJ_ERR_UNSUPPORTED, "too many caches");
-  const int64_t per_block = (a.capacity + cluster - 1) / cluster;
-  c.slice = (int)(std::max<int64_t>(1, (per_block + kThreads - 1) / kThreads) * kThreads);
-  c.staged = c.slice <= kMaxStagedKeys;
-  const int smem = c.staged ? (c.slice + c.slice / 32) * 4 : 0;
-  if (int rc = launch_choose(c, caches, cluster, smem, stream)) return rc;
+  const int64_t threads = (int64_t)cluster * kThreads;
+  c.per = (int)std::max<int64_t>(1, (a.capacity + threads - 1) / threads);
+  int rc = c.per <= 2                   ? launch_choose<2>(c, caches, cluster, stream)
+           : c.per <= 8                 ? launch_choose<8>(c, caches, cluster, stream)
+           : c.per <= kMaxKeysPerThread ? launch_choose<kMaxKeysPerThread>(c, caches, cluster, stream)
+                                        : launch_choose<0>(c, caches, cluster, stream);
+  if (rc) return rc;
   CopyParams p{};
   p.k = static_cast<const uint16_t*>(a.k_cache);
   p.v = static_cast<const uint16_t*>(a.v_cache);

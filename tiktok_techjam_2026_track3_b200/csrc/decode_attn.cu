@@ -4,19 +4,23 @@
 //   o_i = sum_u 2^(s_u - lse_i) v_u,   lse_i = log2 sum_u 2^s_u   (s = scale log2(e) q.k)
 // and joins as  o = sum_i 2^(lse_i - lse) o_i,  lse = log2 sum_i 2^lse_i.
 //
-// Ranges of the caches: one block per (sequence, key / value head, range), bound by
-// the cache's bytes.  A group has few rows (group heads), so the products run on
-// 16-row warp tiles: four warps take 16 or 32 keys in turn, each through its own
-// ring of asynchronous copies (no block barrier in the loop), its own running
-// maximum, sum and output; the block joins its warps at the end.  Rows of the
-// cache past the length are never read: their copies are zero-filled.
+// Caches: bound by their bytes, so the work is cut by bytes.  The steps (16
+// keys of one cache and head) of all caches form one line, in order; each warp of a
+// fixed grid takes an equal stretch of it, whatever the lengths, and streams it
+// through its own ring of asynchronous copies (no block barrier, the ring runs on
+// across cache boundaries).  Where a stretch enters and leaves a cache it leaves a
+// partial result.  A group has few rows (group heads), so the products run on warp
+// tiles of 8 or 16 rows.  Cache rows past the length are never read: their copies are
+// zero-filled.  (One block per cache range of at most 1024 keys, joined through
+// shared memory, took 36 us where the line takes LINE_UNGROUPED for 33 sequences of
+// up to 2100 keys, 16 heads of 64: a range's start and end cost as much as its keys.)
 //
-// Ranges of the prefix: with many rows (batch x group) the 128-row tensor-core
-// kernel (launch_prefix_parts), which reads the prefix once for up to 256 rows;
-// with few, blocks of the cache kernel whose rows belong to several sequences.
+// Prefix: with many rows (batch x group) the 128-row tensor-core kernel
+// (launch_prefix_parts), which reads the prefix once for up to 256 rows; with few,
+// the prefix's steps, a row tile of the batch at a time, come first in the same line.
 //
-// Then one kernel joins the ranges and, with key_weights, turns the stored scores
-// into probabilities with the rows' final lse and adds them up over the group.
+// Then one kernel joins the partial results and, with key_weights, turns the stored
+// scores into probabilities with the rows' final lse and adds them up over the group.
 #include <algorithm>
 #include <atomic>
 
@@ -27,42 +31,60 @@
 namespace ttj {
 namespace {
 
-constexpr int kRows = 16;    // rows of a warp tile
 constexpr int kWarps = 4;
 constexpr int kJoinThreads = 256;
 constexpr int kWeightSpan = 1024;  // cached keys per join block
+constexpr int kMinSteps = 2;       // of a stretch
 
-template <int HD>
-struct RangeSmem {
-  static constexpr int kKeys = HD == 64 ? 32 : 16;   // per warp step
-  static constexpr int kStages = 3;
-  static constexpr int kRowBytes = HD * 2;
-  static constexpr int kTensorBytes = kKeys * kRowBytes;
+// NR: row tiles of 8 (group heads) that a warp carries, 1 or 2.
+template <int HD, int NR>
+struct LineShape {
+  static constexpr int kKeys = 16;                       // per step
+  static constexpr int kStages = HD == 64 ? 4 : 3;
+  static constexpr int kTensorBytes = kKeys * HD * 2;
   static constexpr int kStageBytes = 2 * kTensorBytes;   // K and V
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kTotal = kRing + 2 * kWarps * kRows * 4;
-  static_assert(kWarps * kRows * HD * 4 <= kRing, "the warps' outputs reuse the ring");
+  static constexpr int kTotal = kWarps * kStages * kStageBytes;
+  static constexpr int kBlocksPerSm = HD == 256 ? 1 : (HD == 64 ? 3 : 2);
 };
+constexpr int kStepKeys = 16;
+int line_blocks_per_sm(int64_t hd) { return hd > 128 ? 1 : (hd > 64 ? 2 : 3); }
 
-// How the step is cut into ranges (host).
+// How the step is cut (host).
 struct Cuts {
-  bool prefix_tiles;        // prefix on the 128-row tensor-core kernel
-  int prefix_parts, prefix_keys;
-  int cache_parts, cache_keys;
-  int parts() const { return prefix_parts + cache_parts; }
+  bool prefix_tiles;        // prefix on the 128-row tensor-core kernel, in
+  int tile_parts, tile_keys;  // tile_parts ranges of tile_keys keys
+  int blocks;               // of the line's grid; workers = blocks * kWarps / heads
+  int tile_rows;            // rows of a warp's tile, 8 or 16
+  int prefix_row_tiles;     // row tiles of the batch x group rows when the line has the prefix, else 0
+  int cache_row_tiles;      // of a group
+  int heads;                // consecutive key / value heads that a worker's warps take side by side
+  int64_t units;            // (heads, row tile) of the prefix, (sequence, heads, row tile) of the caches
+  int pitch;                // rows of a partial result
 };
 
-struct RangeParams {
+// The line: positions [0, prefix_steps * prefix units) of the prefix, then the
+// caches' sequence by sequence, `heads` heads at a time.  A worker is as many warps,
+// one per head: in the usual [rows][heads][head_dim] layout they read neighbouring
+// pieces of the same rows at about the same time, which DRAM pages reward.  A partial
+// result's index is its unit plus its worker (along the line one of the two grows
+// from each to the next), then its head.
+struct LineParams {
   const void *q, *pk, *pv, *kc, *vc;
   const int32_t* lengths;
-  float *part_o, *part_lse, *scores;   // scores: [B][Hq][score_pitch] of the cached keys, or null
+  float *part_o, *part_lse;            // [units + workers][heads][pitch][hd], [units + workers][heads][pitch]
+  int64_t* before;                     // [B + 2] steps per (head, row tile) of the sequences before, of all, and the stretch
+  float* scores;                       // [B][Hq][score_pitch] of the cached keys, or null
   int64_t q_seq, q_head, pk_row, pk_head, pv_row, pv_head, kc_seq, kc_row, kc_head, vc_seq, vc_row, vc_head;
   int64_t score_pitch;
-  int batch, prefix, capacity, num_heads, kv_heads, group, hd;
-  int prefix_blocks;        // blocks of the prefix's ranges, before those of the caches
-  int prefix_row_tiles, prefix_keys, prefix_parts, cache_row_tiles, cache_keys;
+  int batch, prefix, capacity, num_heads, head_groups, heads, group, hd;  // kv heads = head_groups * heads
+  int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch;
   float scale_log2;
 };
+
+__host__ __device__ inline int64_t stretch_of(int64_t total_steps, int workers) {
+  const int64_t q = (total_steps + workers - 1) / workers;
+  return q < kMinSteps ? kMinSteps : q;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -92,98 +114,203 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16-byte chunk c of row r within a [rows][HD] tile, swizzled so that eight rows'
-// equal chunks fall into different banks.
-template <int HD>
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4));
+// Transpose of an 8 x 8 matrix of 16-bit elements held one row per four lanes.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kWarps * 32)
-range_kernel(const RangeParams p) {
-  using L = RangeSmem<HD>;
+// Steps of sequence b per (head, row tile).
+__device__ __forceinline__ int seq_steps(const LineParams& p, int64_t b) {
+  return (min(max(__ldg(p.lengths + b), 0), p.capacity) + kStepKeys - 1) / kStepKeys;
+}
+
+// A place in the line: unit, sequence, head group, row tile, the key of the next step
+// and the unit's keys.
+struct Place {
+  int64_t unit, b;
+  int hg, rt, key, keys;
+  bool cached;
+};
+
+// The products are transposed, S^T = K Q^T and O^T = V^T P^T, so that the keys (then
+// the dimensions) fill the 16-row side of the matrix instruction and 8 heads its
+// narrow side: a group of up to 8 pays for 8 rows, not 16.  S^T's accumulators
+// become P^T's operand by two 8 x 8 register transposes per 16 keys.
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(kWarps * 32, LineShape<HD, NR>::kBlocksPerSm)
+line_kernel(const LineParams p) {
+  using L = LineShape<HD, NR>;
   constexpr int kKeys = L::kKeys, kStages = L::kStages;
   constexpr int kChunks = HD / 8;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kRows = 8 * NR;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int64_t s_before[kWarps * 32 + 1];  // steps before each thread's sequences, and of all
   grid_dependency_wait();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, kq = lane & 3;
 
-  // Which rows and keys: row r of the block is query head h0 + (i % group) of
-  // sequence i / group for i = row0 + r < rows.
-  const T *kbase, *vbase;
-  int64_t krow, vrow, row0, rows;
-  int kvh, keys_from, keys_to, part;
-  bool cached = false;
-  int64_t blk = blockIdx.x;
-  if (blk < p.prefix_blocks) {
-    part = (int)(blk / (p.kv_heads * p.prefix_row_tiles));
-    const int rest = (int)(blk - (int64_t)part * p.kv_heads * p.prefix_row_tiles);
-    kvh = rest / p.prefix_row_tiles;
-    row0 = (int64_t)(rest - kvh * p.prefix_row_tiles) * kRows;
-    rows = (int64_t)p.batch * p.group;
-    kbase = static_cast<const T*>(p.pk) + kvh * p.pk_head;
-    vbase = static_cast<const T*>(p.pv) + kvh * p.pv_head;
-    krow = p.pk_row;
-    vrow = p.pv_row;
-    keys_from = part * p.prefix_keys;
-    keys_to = min(keys_from + p.prefix_keys, p.prefix);
-  } else {
-    blk -= p.prefix_blocks;
-    const int64_t per_part = (int64_t)p.batch * p.kv_heads * p.cache_row_tiles;
-    part = (int)(blk / per_part);
-    int64_t rest = blk - part * per_part;
-    const int64_t b = rest / (p.kv_heads * p.cache_row_tiles);
-    rest -= b * p.kv_heads * p.cache_row_tiles;
-    kvh = (int)(rest / p.cache_row_tiles);
-    row0 = b * p.group + (rest - kvh * p.cache_row_tiles) * kRows;
-    rows = (b + 1) * p.group;
-    kbase = static_cast<const T*>(p.kc) + b * p.kc_seq + kvh * p.kc_head;
-    vbase = static_cast<const T*>(p.vc) + b * p.vc_seq + kvh * p.vc_head;
-    krow = p.kc_row;
-    vrow = p.vc_row;
-    keys_from = part * p.cache_keys;
-    keys_to = min(keys_from + p.cache_keys, min(max(__ldg(p.lengths + b), 0), p.capacity));
-    part += p.prefix_parts;
-    cached = true;
-  }
-  // row index in [B][Hq] of block row r, or -1
-  auto out_row = [&](int r) -> int64_t {
-    const int64_t i = row0 + r;
-    if (i >= rows) return -1;
-    const int64_t b = i / p.group;
-    return b * p.num_heads + kvh * p.group + (i - b * p.group);
-  };
-  const int64_t part_row0 = (int64_t)part * p.batch * p.num_heads;
-  if (keys_from >= keys_to) {  // nothing in this range: the join skips it
-    if (threadIdx.x < kRows) {
-      const int64_t at = out_row(threadIdx.x);
-      if (at >= 0) p.part_lse[part_row0 + at] = -INFINITY;
+  // Steps before each thread's run of consecutive sequences.
+  const int64_t run = ((int64_t)p.batch + kWarps * 32 - 1) / (kWarps * 32);
+  const int64_t b0 = min(threadIdx.x * run, (int64_t)p.batch), b1 = min(b0 + run, (int64_t)p.batch);
+  {
+    int64_t sum = 0;
+    for (int64_t b = b0; b < b1; ++b) sum += seq_steps(p, b);
+    int64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
     }
-    return;
+    if (lane == 31) s_before[warp] = inc;
+    __syncthreads();
+    int64_t base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += s_before[w];
+      all += s_before[w];
+    }
+    __syncthreads();
+    s_before[threadIdx.x] = base + inc - sum;
+    if (threadIdx.x == 0) s_before[kWarps * 32] = all;
+    if (blockIdx.x == 0) {  // for the join
+      int64_t at = base + inc - sum;
+      for (int64_t b = b0; b < b1; ++b) {
+        p.before[b] = at;
+        at += seq_steps(p, b);
+      }
+      if (threadIdx.x == 0) {
+        p.before[p.batch] = all;
+        p.before[p.batch + 1] =
+            stretch_of((int64_t)p.prefix_steps * p.prefix_units + all * p.head_groups * p.cache_row_tiles,
+                       gridDim.x * kWarps / p.heads);
+      }
+    }
+    __syncthreads();
   }
+  const int64_t per_step = (int64_t)p.head_groups * p.cache_row_tiles;  // units of a sequence
+  const int64_t prefix_total = (int64_t)p.prefix_steps * p.prefix_units;
+  const int64_t total = prefix_total + s_before[kWarps * 32] * per_step;
+  const int side = warp % p.heads;       // this warp's head among the worker's
+  const int64_t worker = (int64_t)blockIdx.x * (kWarps / p.heads) + warp / p.heads;
+  const int64_t stretch = stretch_of(total, gridDim.x * kWarps / p.heads);
+  const int64_t from = worker * stretch;
+  const int steps = (int)min(stretch, total - from);
+  if (steps <= 0) return;  // uniform over the warp; no block barrier follows
 
-  const int steps_all = (keys_to - keys_from + kKeys - 1) / kKeys;
-  const int steps = (steps_all - warp + kWarps - 1) / kWarps;  // this warp's: warp, warp + kWarps, ...
-  uint8_t* ring = smem + warp * kStages * L::kStageBytes;
-  const uint32_t ring_s = smem_u32(ring);
+  Place at;
+  if (from < prefix_total) {
+    at.cached = false;
+    at.unit = from / p.prefix_steps;
+    at.hg = (int)(at.unit / p.prefix_row_tiles);
+    at.rt = (int)(at.unit - (int64_t)at.hg * p.prefix_row_tiles);
+    at.key = (int)(from - at.unit * p.prefix_steps) * kKeys;
+    at.keys = p.prefix;
+    at.b = -1;
+  } else {
+    const int64_t line = from - prefix_total;
+    const int64_t want = line / per_step;  // the sequence b with before[b] <= want < before[b + 1]
+    int64_t t = -1;                        // last thread's run starting at or before it
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) t += __popc(__ballot_sync(0xffffffffu, s_before[32 * w + lane] <= want));
+    int64_t b = t * run, base = s_before[t];
+    for (;;) {  // 32 sequences at a time
+      const int64_t mine = b + lane;
+      const int64_t n = mine < p.batch ? seq_steps(p, mine) : 0;
+      int64_t inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, base + inc > want);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1;
+        b += l;
+        base += __shfl_sync(0xffffffffu, inc - n, l);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+      b += 32;
+    }
+    const int64_t n = seq_steps(p, b);
+    const int64_t in_seq = line - base * per_step;
+    const int64_t u = in_seq / n;
+    at.cached = true;
+    at.b = b;
+    at.unit = p.prefix_units + b * per_step + u;
+    at.hg = (int)(u / p.cache_row_tiles);
+    at.rt = (int)(u - (int64_t)at.hg * p.cache_row_tiles);
+    at.key = (int)(in_seq - u * n) * kKeys;
+    at.keys = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  }
+  // The place after a step; only called while steps remain.
+  auto advance = [&](Place& x) {
+    x.key += kKeys;
+    if (x.key < x.keys) return;
+    x.key = 0;
+    ++x.unit;
+    if (x.cached) {
+      if (++x.rt < p.cache_row_tiles) return;
+      x.rt = 0;
+      if (++x.hg < p.head_groups) return;
+    } else {
+      if (++x.rt < p.prefix_row_tiles) return;
+      x.rt = 0;
+      if (++x.hg < p.head_groups) return;
+      x.cached = true;
+    }
+    x.hg = 0;
+    do {
+      ++x.b;
+      x.keys = min(max(__ldg(p.lengths + x.b), 0), p.capacity);
+    } while (x.keys == 0);
+    x.unit = p.prefix_units + x.b * per_step;
+  };
+
+  const uint32_t ring_s = smem_u32(smem) + warp * kStages * L::kStageBytes;
+  // Copies: lane -> 16-byte chunk ld_chunk of rows ld_row, ld_row + kRowsPerPass, ...;
+  // chunk c of row r lies at c ^ (r & 7), so that eight rows' equal chunks fall into
+  // different banks.
   const int ld_chunk = lane % kChunks, ld_row = lane / kChunks;
   constexpr int kRowsPerPass = 32 / kChunks;
   const bool ld_col = ld_chunk * 8 < p.hd;
+  const uint32_t ld_dst = ring_s + ld_row * (HD * 2) + ((ld_chunk ^ ld_row) << 4);
+  Place next = at;  // where the loads are
+  const T *kp = nullptr, *vp = nullptr;  // this lane's first element of the next step
+  bool moved = true;                     // `next` has entered another unit
+  int64_t kstep = 0, vstep = 0;
   auto load = [&](int i) {
     if (i < steps) {
-      const int key0 = keys_from + (warp + i * kWarps) * kKeys;
-      const uint32_t dst = ring_s + (i % kStages) * L::kStageBytes;
+      if (moved) {
+        kstep = next.cached ? p.kc_row : p.pk_row;
+        vstep = next.cached ? p.vc_row : p.pv_row;
+        kp = next.cached ? static_cast<const T*>(p.kc) + next.b * p.kc_seq + (next.hg * p.heads + side) * p.kc_head
+                         : static_cast<const T*>(p.pk) + (next.hg * p.heads + side) * p.pk_head;
+        vp = next.cached ? static_cast<const T*>(p.vc) + next.b * p.vc_seq + (next.hg * p.heads + side) * p.vc_head
+                         : static_cast<const T*>(p.pv) + (next.hg * p.heads + side) * p.pv_head;
+        kp += (next.key + ld_row) * kstep + ld_chunk * 8;
+        vp += (next.key + ld_row) * vstep + ld_chunk * 8;
+      }
+      const int left = next.keys - next.key - ld_row;
+      const uint32_t dst = ld_dst + (i % kStages) * L::kStageBytes;
 #pragma unroll
       for (int r = 0; r < kKeys; r += kRowsPerPass) {
-        const int row = r + ld_row;
-        const bool ok = ld_col && key0 + row < keys_to;
-        const int64_t key = ok ? key0 + row : keys_from;
-        const int col = ok ? ld_chunk * 8 : 0;
-        cp_async16(dst + tile_at<HD>(row, ld_chunk), kbase + key * krow + col, ok);
-        cp_async16(dst + L::kTensorBytes + tile_at<HD>(row, ld_chunk), vbase + key * vrow + col, ok);
+        // rows past the end are filled with zeros (their address, this lane's
+        // first row or row 0 of the unit's keys, is not read)
+        const bool ok = ld_col && r < left;
+        const uint32_t to = (dst ^ ((r & 7) << 4)) + r * (HD * 2);
+        cp_async16(to, ok ? kp + r * kstep : p.q, ok);
+        cp_async16(to + L::kTensorBytes, ok ? vp + r * vstep : p.q, ok);
+      }
+      if (i + 1 < steps) {
+        const int64_t unit = next.unit;
+        advance(next);
+        moved = next.unit != unit;
+        kp += kKeys * kstep;
+        vp += kKeys * vstep;
       }
     }
     cp_async_commit();
@@ -191,265 +318,364 @@ range_kernel(const RangeParams p) {
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load(i);
 
-  // Q fragments straight from global memory: rows g and g + 8, columns 16 kk + 2 kq (+ 8)
-  uint32_t qf[HD / 16][4];
-  {
-    const int64_t i0 = row0 + g, i1 = row0 + g + 8;
-    auto q_row = [&](int64_t i) -> const T* {
-      if (i >= rows) return nullptr;
-      const int64_t b = i / p.group;
-      return static_cast<const T*>(p.q) + b * p.q_seq + (kvh * p.group + (i - b * p.group)) * p.q_head;
-    };
-    const T *qa = q_row(i0), *qb = q_row(i1);
-#pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const T* src = (e & 1) ? qb : qa;
-        const int col = 16 * kk + 2 * kq + (e >> 1) * 8;
-        qf[kk][e] = (src != nullptr && col < p.hd) ? __ldg(reinterpret_cast<const uint32_t*>(src + col)) : 0u;
-      }
-    }
-  }
-  float o[HD / 8][4];
-#pragma unroll
-  for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const int64_t at_a = out_row(g), at_b = out_row(g + 8);
-  const bool both = rows - row0 > 8;  // rows 8..15 hold heads
-
+  // Fragments of this lane: Q^T (B side) head g, dimensions 16 kk + 2 kq (+ 8);
+  // S^T keys g and g + 8, heads 2 kq and 2 kq + 1; O^T dimensions 16 n + g (+ 8),
+  // the same heads; per row tile.
+  uint32_t qf[NR][HD / 16][2];
+  float o[NR][HD / 16][4];
+  float m[NR][2], l[NR][2];
+  int64_t at_row[NR][2];         // output rows ([B][Hq]) of heads 2 kq and 2 kq + 1, or -1
+  bool fresh = true;
+  // operand addresses within a stage, before the step's and column's offset
+  const int r7 = lane & 7;
+  const uint32_t k_at = (r7 + ((lane >> 3) & 1) * 8) * (HD * 2) + (((lane >> 4) ^ r7) << 4);
+  const uint32_t v_at = L::kTensorBytes + (r7 + (lane >> 4) * 8) * (HD * 2) + ((((lane >> 3) & 1) ^ r7) << 4);
   for (int i = 0; i < steps; ++i) {
+    if (fresh) {
+      // The unit's rows: tile row r is row i0 + r of the batch x group rows.
+      const int64_t i0 = (at.cached ? at.b * p.group : 0) + at.rt * kRows;
+      const int64_t end = at.cached ? (at.b + 1) * p.group : (int64_t)p.batch * p.group;
+      auto row_of = [&](int r, int64_t& b, int& head) -> bool {
+        const int64_t x = i0 + r;
+        b = at.cached ? at.b : x / p.group;
+        head = (at.hg * p.heads + side) * p.group + (int)(x - b * p.group);
+        return x < end;
+      };
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        int64_t b;
+        int head;
+        const bool ok = row_of(8 * t + g, b, head);
+        const T* src = static_cast<const T*>(p.q) + b * p.q_seq + head * p.q_head + 2 * kq;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[t][kk][e] = ok && 16 * kk + 8 * e < p.hd ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * kk + 8 * e)) : 0u;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          at_row[t][e] = row_of(8 * t + 2 * kq + e, b, head) ? b * p.num_heads + head : -1;
+          m[t][e] = -INFINITY;
+          l[t][e] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < HD / 16; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
+      }
+      fresh = false;
+    }
     cp_async_wait<kStages - 2>();
     __syncwarp();
     load(i + kStages - 1);
-    const int key0 = keys_from + (warp + i * kWarps) * kKeys;
-    const uint32_t sk = ring_s + (i % kStages) * L::kStageBytes, sv = sk + L::kTensorBytes;
-    float s[kKeys / 8][4];
+    const int left = at.keys - at.key;
+    const uint32_t stage = ring_s + (i % kStages) * L::kStageBytes;
+    float s[NR][4];
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n)
+    for (int t = 0; t < NR; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk)
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      uint32_t a[4];
+      ldmatrix_x4(a, (stage + k_at) ^ (kk << 5));
 #pragma unroll
-      for (int n = 0; n < kKeys / 16; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4(b, sk + tile_at<HD>(16 * n + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
-        mma_16x8x16<T>(s[2 * n], qf[kk], b[0], b[1]);
-        mma_16x8x16<T>(s[2 * n + 1], qf[kk], b[2], b[3]);
+      for (int t = 0; t < NR; ++t) mma_16x8x16<T>(s[t], a, qf[t][kk][0], qf[t][kk][1]);
+    }
+    uint32_t pf[NR][2];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][e] *= p.scale_log2;   // s[t][e]: key g + 8 (e >> 1), head 2 kq + (e & 1)
+      if (left < kKeys) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = g + 8 * (e >> 1) < left ? s[t][e] : -INFINITY;
       }
-    // s[n][e]: row g + 8 (e >> 1), key 8 n + 2 kq + (e & 1)
-    float mx[2] = {-INFINITY, -INFINITY};
+      if (at.cached && p.scores != nullptr) {
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool ok = key0 + 8 * n + 2 * kq + (e & 1) < keys_to;
-        s[n][e] = ok ? s[n][e] * p.scale_log2 : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      }
-    if (cached && p.scores != nullptr) {
-#pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n) {
-        const int key = key0 + 8 * n + 2 * kq;
-        if (key < keys_to) {  // the pitch is even: the pair's second key stays in the row
-          if (at_a >= 0) *reinterpret_cast<float2*>(p.scores + at_a * p.score_pitch + key) = make_float2(s[n][0], s[n][1]);
-          if (at_b >= 0) *reinterpret_cast<float2*>(p.scores + at_b * p.score_pitch + key) = make_float2(s[n][2], s[n][3]);
+        for (int e = 0; e < 4; ++e) {
+          const int col = g + 8 * (e >> 1);
+          if (at_row[t][e & 1] >= 0 && col < left) p.scores[at_row[t][e & 1] * p.score_pitch + at.key + col] = s[t][e];
         }
       }
-    }
-    float alpha[2], ref[2];
+      float alpha[2], ref[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-      const float mn = mx[e] > m[e] + 8.f ? mx[e] : m[e];  // the reference moves lazily: P <= 2^8
-      ref[e] = mn == -INFINITY ? 0.f : mn;
-      alpha[e] = fast_exp2(m[e] - ref[e]);
-      m[e] = mn;
-      l[e] *= alpha[e];
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[t][e], s[t][e + 2]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = mx > m[t][e] + 8.f ? mx : m[t][e];  // the reference moves lazily: P <= 2^8
+        ref[e] = mn == -INFINITY ? 0.f : mn;
+        alpha[e] = fast_exp2(m[t][e] - ref[e]);
+        m[t][e] = mn;
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
+        for (int e = 0; e < 2; ++e) l[t][e] *= alpha[e];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
-    }
-    uint32_t pf[kKeys / 16][4];
+        for (int n = 0; n < HD / 16; ++n)
 #pragma unroll
-    for (int n = 0; n < kKeys / 8; ++n) {
-      const float e0 = fast_exp2(s[n][0] - ref[0]), e1 = fast_exp2(s[n][1] - ref[0]);
-      l[0] += e0 + e1;
-      pf[n >> 1][(n & 1) * 2] = Pack<T>::two(e0, e1);
-      if (both) {
-        const float e2 = fast_exp2(s[n][2] - ref[1]), e3 = fast_exp2(s[n][3] - ref[1]);
-        l[1] += e2 + e3;
-        pf[n >> 1][(n & 1) * 2 + 1] = Pack<T>::two(e2, e3);
-      } else {
-        pf[n >> 1][(n & 1) * 2 + 1] = 0u;
+          for (int e = 0; e < 4; ++e) o[t][n][e] *= alpha[e & 1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // keys g, then g + 8
+        const float e0 = fast_exp2(s[t][2 * h] - ref[0]), e1 = fast_exp2(s[t][2 * h + 1] - ref[1]);
+        l[t][0] += e0;
+        l[t][1] += e1;
+        pf[t][h] = movmatrix_trans(Pack<T>::two(e0, e1));  // head g, keys 8 h + 2 kq, 8 h + 2 kq + 1
       }
     }
 #pragma unroll
-    for (int kk = 0; kk < kKeys / 16; ++kk)
+    for (int n = 0; n < HD / 16; ++n) {
+      uint32_t a[4];
+      ldmatrix_x4_trans(a, (stage + v_at) ^ (n << 5));
 #pragma unroll
-      for (int n = 0; n < HD / 16; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, sv + tile_at<HD>(16 * kk + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
-        mma_16x8x16<T>(o[2 * n], pf[kk], b[0], b[1]);
-        mma_16x8x16<T>(o[2 * n + 1], pf[kk], b[2], b[3]);
-      }
-  }
-
-  // join the warps: o and l rescaled to the block's maximum
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-  }
-  cp_async_wait<0>();
-  float* s_m = reinterpret_cast<float*>(smem + L::kRing);
-  float* s_l = s_m + kWarps * kRows;
-  if (kq == 0) {
-    s_m[warp * kRows + g] = m[0];
-    s_m[warp * kRows + g + 8] = m[1];
-    s_l[warp * kRows + g] = l[0];
-    s_l[warp * kRows + g + 8] = l[1];
-  }
-  __syncthreads();  // every warp has left its ring
-  float* s_o = reinterpret_cast<float*>(smem);  // [kWarps][kRows][HD]
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int r = g + 8 * e;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * kRows + r]);
-    const float f = m[e] == -INFINITY ? 0.f : fast_exp2(m[e] - top);
-#pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
-      *reinterpret_cast<float2*>(s_o + (warp * kRows + r) * HD + 8 * n + 2 * kq) =
-          make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * (HD / 4); i += kWarps * 32) {
-    const int r = i / (HD / 4), col = (i - r * (HD / 4)) * 4;
-    const int64_t at = out_row(r);
-    if (at < 0) break;  // rows ascend with i
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w * kRows + r]);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = s_m[w * kRows + r];
-      if (mw != -INFINITY) sum += s_l[w * kRows + r] * fast_exp2(mw - top);
-      const float4 x = *reinterpret_cast<const float4*>(s_o + (w * kRows + r) * HD + col);
-      v.x += x.x;
-      v.y += x.y;
-      v.z += x.z;
-      v.w += x.w;
+      for (int t = 0; t < NR; ++t) mma_16x8x16<T>(o[t][n], a, pf[t][0], pf[t][1]);
     }
-    const float inv = 1.f / sum;
-    if (col < p.hd)
-      *reinterpret_cast<float4*>(p.part_o + (part_row0 + at) * p.hd + col) =
-          make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    if (col == 0) p.part_lse[part_row0 + at] = top + log2f(sum);
+    if (left <= kKeys || i + 1 == steps) {  // the stretch leaves this unit
+#pragma unroll
+      for (int t = 0; t < NR; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[t][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          if (at_row[t][e] < 0) continue;
+          const int64_t row = ((at.unit + worker) * p.heads + side) * p.pitch + 8 * t + 2 * kq + e;
+          const float inv = 1.f / sum;
+          float* out = p.part_o + row * p.hd + g;
+#pragma unroll
+          for (int n = 0; n < HD / 16; ++n) {
+            if (16 * n < p.hd) out[16 * n] = o[t][n][e] * inv;
+            if (16 * n + 8 < p.hd) out[16 * n + 8] = o[t][n][e + 2] * inv;
+          }
+          if (g == 0) p.part_lse[row] = m[t][e] + log2f(sum);
+        }
+      fresh = true;
+    }
+    if (i + 1 < steps) advance(at);
   }
 }
 
 struct JoinParams {
-  const float *part_o, *part_lse, *scores, *key_weights;
+  const float *tile_o, *tile_lse;      // [tile_parts][B][Hq][hd], [tile_parts][B][Hq]
+  const float *part_o, *part_lse;      // the line's
+  const int64_t* before;
+  const float *scores, *key_weights;
   float* key_weights_out;
   void* out;
   const int32_t* lengths;
-  int64_t score_pitch;
-  int batch, capacity, num_heads, kv_heads, group, hd, parts;
+  int64_t score_pitch, rows, out_blocks;
+  int spans;                           // of kWeightSpan cached keys
+  int capacity, batch, num_heads, kv_heads, group, hd, tile_parts;
+  int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch, tile_rows;
+  int heads_shift;                     // log2 of the line's heads
 };
 
-// One block per (sequence, key / value head) and span of cached keys: lse of the
-// group's rows from the ranges'; the first span's block writes the output rows.
+// a / b for a, b >= 0: the 32-bit division where it suffices (a 64-bit one is a
+// long dependent chain).
+__device__ __forceinline__ int64_t div_of(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// Where the partial results of one output row are: tile_parts of the prefix's
+// tensor-core ranges, then the line's, consecutive per unit.
+struct RowParts {
+  int64_t row, prefix_first, cache_first;  // first partial row (index * pitch + tile row)
+  int prefix_count, cache_count;
+};
+
+__device__ __forceinline__ RowParts row_parts(const JoinParams& p, int64_t b, int head) {
+  RowParts x;
+  x.row = b * p.num_heads + head;
+  const int kvh = (uint32_t)head / (uint32_t)p.group, in_group = head - kvh * p.group;
+  const int hg = kvh >> p.heads_shift, side = kvh - (hg << p.heads_shift);
+  const int64_t per_seq = (int64_t)(p.kv_heads >> p.heads_shift) * p.cache_row_tiles;
+  const int64_t prefix_total = (int64_t)p.prefix_steps * p.prefix_units;
+  const int64_t before = p.before[b], steps = p.before[b + 1] - before;
+  const int64_t stretch = p.before[p.batch + 1];
+  auto locate = [&](int64_t unit, int64_t from, int64_t n, int tile_row, int64_t& first, int& count) {
+    const int64_t w0 = div_of(from, stretch), w1 = div_of(from + max(n, (int64_t)1) - 1, stretch);
+    first = (((unit + w0) << p.heads_shift) + side) * p.pitch + tile_row;
+    count = n > 0 ? (int)(w1 - w0 + 1) : 0;
+  };
+  x.prefix_count = 0;
+  x.prefix_first = 0;
+  const int rt_shift = p.tile_rows == 16 ? 4 : 3;
+  if (p.prefix_units > 0) {
+    const int64_t i = b * p.group + in_group;
+    const int64_t unit = hg * p.prefix_row_tiles + (i >> rt_shift);
+    locate(unit, unit * p.prefix_steps, p.prefix_steps, (int)(i & (p.tile_rows - 1)), x.prefix_first, x.prefix_count);
+  }
+  const int64_t u = (int64_t)hg * p.cache_row_tiles + (in_group >> rt_shift);
+  locate(p.prefix_units + b * per_seq + u, prefix_total + before * per_seq + u * steps, steps,
+         in_group & (p.tile_rows - 1), x.cache_first, x.cache_count);
+  return x;
+}
+
+// i-th partial result: its lse and (float) offset of its output from `tile_o`.
+__device__ __forceinline__ float part_at(const JoinParams& p, const RowParts& x, int i, int64_t& offset) {
+  if (i < p.tile_parts) {
+    const int64_t r = i * p.rows + x.row;
+    offset = r * p.hd;
+    return p.tile_lse[r];
+  }
+  i -= p.tile_parts;
+  const int64_t next = (int64_t)p.pitch << p.heads_shift;
+  const int64_t r = i < x.prefix_count ? x.prefix_first + i * next : x.cache_first + (i - x.prefix_count) * next;
+  offset = (p.part_o - p.tile_o) + r * p.hd;
+  return p.part_lse[r];
+}
+
+// lse of a row over all its partial results (the whole warp; -inf without any key).
+__device__ __forceinline__ float row_lse(const JoinParams& p, const RowParts& x, int count) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY, sum = 0.f;
+  int64_t unused;
+  for (int i = lane; i < count; i += 32) {
+    const float v = part_at(p, x, i, unused);
+    const float t = fmaxf(top, v);
+    if (v != -INFINITY) sum = sum * fast_exp2(top - t) + fast_exp2(v - t);
+    top = t;
+  }
+  float all = top;
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, w));
+  sum = sum == 0.f ? 0.f : sum * fast_exp2(top - all);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  return all + log2f(sum);
+}
+
+// The first out_blocks blocks write the output, one warp per row, in one pass over
+// its partial results; the others the weights of a span of cached keys of one
+// (sequence, key / value head).
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  __shared__ float s_lse[kMaxGroup];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.x / p.kv_heads;
-  const int kvh = (int)(blockIdx.x - b * p.kv_heads);
-  const int64_t row0 = b * p.num_heads + kvh * p.group;
-  const int64_t rows = (int64_t)p.batch * p.num_heads;
-  for (int r = warp; r < p.group; r += kJoinThreads / 32) {
-    float top = -INFINITY;
-    for (int i = lane; i < p.parts; i += 32) top = fmaxf(top, p.part_lse[i * rows + row0 + r]);
+  if (blockIdx.x < p.out_blocks) {
+    const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 32) + warp;
+    if (row >= p.rows) return;
+    const int64_t b = div_of(row, p.num_heads);
+    const RowParts x = row_parts(p, b, (int)(row - b * p.num_heads));
+    const int count = p.tile_parts + x.prefix_count + x.cache_count;
+    for (int col0 = 0; col0 < p.hd; col0 += 128) {
+      const int col = col0 + lane * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float top = -INFINITY, sum = 0.f;
+      for (int i0 = 0; i0 < count; i0 += 32) {
+        int64_t offset = 0;
+        const float lse = i0 + lane < count ? part_at(p, x, i0 + lane, offset) : -INFINITY;
+        float now = lse;
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    float sum = 0.f;
-    for (int i = lane; i < p.parts; i += 32) {
-      const float v = p.part_lse[i * rows + row0 + r];
-      if (v != -INFINITY) sum += fast_exp2(v - top);
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    const float lse = top + log2f(sum);  // -inf without any key
-    if (lane == 0) s_lse[r] = lse;
-    if (blockIdx.y == 0) {
-      for (int col = lane * 4; col < p.hd; col += 128) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < p.parts; ++i) {
-          const float li = p.part_lse[i * rows + row0 + r];
-          if (li == -INFINITY) continue;  // an empty range's output is not written
-          const float f = fast_exp2(li - lse);
-          const float4 x = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row0 + r) * p.hd + col);
-          v.x = fmaf(f, x.x, v.x);
-          v.y = fmaf(f, x.y, v.y);
-          v.z = fmaf(f, x.z, v.z);
-          v.w = fmaf(f, x.w, v.w);
+        for (int w = 16; w > 0; w >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, w));
+        now = fmaxf(now, top);
+        const float keep = top == -INFINITY ? 0.f : fast_exp2(top - now);
+        const float f = lse == -INFINITY ? 0.f : fast_exp2(lse - now);
+        top = now;
+        sum = sum * keep + f;
+        v = make_float4(v.x * keep, v.y * keep, v.z * keep, v.w * keep);
+        const int n = min(32, count - i0);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const float fi = __shfl_sync(0xffffffffu, f, i);
+          const int64_t oi = __shfl_sync(0xffffffffu, offset, i);
+          if (col < p.hd) {
+            const float4 y = __ldg(reinterpret_cast<const float4*>(p.tile_o + oi + col));
+            v.x = fmaf(fi, y.x, v.x);
+            v.y = fmaf(fi, y.y, v.y);
+            v.z = fmaf(fi, y.z, v.z);
+            v.w = fmaf(fi, y.w, v.w);
+          }
         }
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (row0 + r) * p.hd + col) =
-            make_uint2(Pack<T>::two(v.x, v.y), Pack<T>::two(v.z, v.w));
       }
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
+      if (col < p.hd)
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * p.hd + col) =
+            make_uint2(Pack<T>::two(v.x * inv, v.y * inv), Pack<T>::two(v.z * inv, v.w * inv));
+    }
+    return;
+  }
+  __shared__ float s_lse[kMaxGroup];
+  int64_t rest = blockIdx.x - p.out_blocks;
+  const int64_t bh = rest / p.spans;
+  const int span = (int)(rest - bh * p.spans);
+  const int64_t b = bh / p.kv_heads;
+  const int kvh = (int)(bh - b * p.kv_heads);
+  const int n = min(max(__ldg(p.lengths + b), 0), p.capacity);
+  const int c0 = span * kWeightSpan + threadIdx.x;
+  constexpr int kPer = kWeightSpan / kJoinThreads;
+  float sum[kPer], w[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int c = c0 + q * kJoinThreads;
+    sum[q] = 0.f;
+    w[q] = c < p.capacity ? __ldg(p.key_weights + bh * p.capacity + c) : 0.f;
+  }
+  if (span * kWeightSpan < n) {  // uniform
+    const float* scores = p.scores + (b * p.num_heads + kvh * p.group) * p.score_pitch;
+    constexpr int kAhead = 4;    // rows whose scores are read before the lse are known
+    float x[kAhead][kPer];
+    auto fetch = [&](int r0) {
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r)
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          const int c = c0 + q * kJoinThreads;
+          x[r][q] = r0 + r < p.group && c < n ? __ldg(scores + (r0 + r) * p.score_pitch + c) : -INFINITY;
+        }
+    };
+    fetch(0);
+    for (int r = warp; r < p.group; r += kJoinThreads / 32) {
+      const RowParts y = row_parts(p, b, kvh * p.group + r);
+      const float lse = row_lse(p, y, p.tile_parts + y.prefix_count + y.cache_count);
+      if (lane == 0) s_lse[r] = lse;
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < p.group; r0 += kAhead) {
+      if (r0 > 0) fetch(r0);
+#pragma unroll
+      for (int r = 0; r < kAhead; ++r)
+        if (r0 + r < p.group) {
+          const float lse = s_lse[r0 + r];
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) sum[q] += fast_exp2(x[r][q] - lse);
+        }
     }
   }
-  if (p.scores == nullptr) return;
-  __syncthreads();
-  const int n = min(max(__ldg(p.lengths + b), 0), p.capacity);
-  const int64_t base = ((int64_t)b * p.kv_heads + kvh) * p.capacity;
-  const int to = min((int)(blockIdx.y + 1) * kWeightSpan, p.capacity);
-  for (int c = blockIdx.y * kWeightSpan + threadIdx.x; c < to; c += kJoinThreads) {
-    float sum = 0.f;
-    if (c < n)
-      for (int r = 0; r < p.group; ++r) sum += fast_exp2(p.scores[(row0 + r) * p.score_pitch + c] - s_lse[r]);
-    p.key_weights_out[base + c] = p.key_weights[base + c] + sum;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int c = c0 + q * kJoinThreads;
+    if (c < p.capacity) p.key_weights_out[bh * p.capacity + c] = w[q] + (c < n ? sum[q] : 0.f);
   }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Ranges for `units` blocks-per-range over `keys` keys: enough blocks to fill the
-// GPU's resident blocks a few times over, ranges of 64 to 1024 keys.
-void cut_ranges(int64_t units, int64_t keys, int& parts, int& part_keys) {
-  if (keys == 0) {
-    parts = 0;
-    part_keys = 64;
-    return;
-  }
-  int64_t n = ceil_div(8 * (int64_t)sm_count(), units);
-  n = std::max(n, ceil_div(keys, 1024));
-  n = std::max<int64_t>(1, std::min(n, ceil_div(keys, 64)));
-  part_keys = (int)(ceil_div(ceil_div(keys, n), 64) * 64);
-  parts = (int)ceil_div(keys, part_keys);
-}
-
 Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads, int64_t kv_heads, int64_t hd) {
   Cuts c{};
   const int64_t group = num_heads / kv_heads, rows = batch * group;
-  cut_ranges(batch * kv_heads * ceil_div(group, kRows), capacity, c.cache_parts, c.cache_keys);
   c.prefix_tiles = prefix > 0 && rows > 32;
-  if (!c.prefix_tiles) {
-    cut_ranges(kv_heads * ceil_div(rows, kRows), prefix, c.prefix_parts, c.prefix_keys);
-    return c;
-  }
+  const int64_t tile = (c.prefix_tiles || prefix == 0 ? group : rows) <= 8 ? 8 : 16;
+  c.tile_rows = (int)tile;
+  c.prefix_row_tiles = prefix > 0 && !c.prefix_tiles ? (int)ceil_div(rows, tile) : 0;
+  c.cache_row_tiles = (int)ceil_div(group, tile);
+  c.heads = kv_heads % 4 == 0 ? 4 : (kv_heads % 2 == 0 ? 2 : 1);
+  const int64_t head_groups = kv_heads / c.heads;
+  c.units = head_groups * c.prefix_row_tiles + batch * head_groups * c.cache_row_tiles;
+  c.pitch = c.prefix_row_tiles > 0 ? (int)tile : (int)std::min<int64_t>(group, tile);
+  // As many blocks as stay resident, and no more than the longest line has work for.
+  const int64_t steps = head_groups * (c.prefix_row_tiles * ceil_div(prefix, kStepKeys) +
+                                       batch * c.cache_row_tiles * ceil_div(capacity, kStepKeys));
+  c.blocks = (int)std::min<int64_t>(line_blocks_per_sm(hd) * (int64_t)sm_count(),
+                                    ceil_div(steps * c.heads, kMinSteps * kWarps));
+  if (!c.prefix_tiles) return c;
   // Persistent blocks, one per SM: the number of ranges with the least time, in key
   // tiles of 128: waves x (tiles of a range + about 2 for its start and end).
   const int64_t units = kv_heads * ceil_div(batch, plan_positions(group, hd)), tiles = ceil_div(prefix, 128);
@@ -460,31 +686,35 @@ Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads,
     const int64_t time = ceil_div(units * n, sm_count()) * (per + 2) * 16 + n;
     if (time < best_time) best_time = time, best = n;
   }
-  c.prefix_keys = (int)(ceil_div(tiles, best) * 128);
-  c.prefix_parts = (int)best;
+  c.tile_keys = (int)(ceil_div(tiles, best) * 128);
+  c.tile_parts = (int)best;
   return c;
 }
 
 struct Workspace {
-  size_t part_o, part_lse, scores, total;  // byte offsets
-  int64_t pitch;
+  size_t tile_o, tile_lse, part_o, part_lse, before, scores, total;  // byte offsets
+  int64_t pitch;                                                     // of the scores
 };
 Workspace workspace_of(const Cuts& c, int64_t batch, int64_t capacity, int64_t num_heads, int64_t hd, bool weights) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   const size_t rows = (size_t)batch * num_heads;
+  const size_t parts = c.blocks > 0 ? (size_t)c.units * c.heads + (size_t)c.blocks * kWarps : 0;
   Workspace w;
   w.pitch = (capacity + 3) / 4 * 4;
-  w.part_o = 0;
-  w.part_lse = up((size_t)c.parts() * rows * hd * 4);
-  w.scores = w.part_lse + up((size_t)c.parts() * rows * 4);
+  w.tile_o = 0;
+  w.tile_lse = w.tile_o + up((size_t)c.tile_parts * rows * hd * 4);
+  w.part_o = w.tile_lse + up((size_t)c.tile_parts * rows * 4);
+  w.part_lse = w.part_o + up(parts * c.pitch * hd * 4);
+  w.before = w.part_lse + up(parts * c.pitch * 4);
+  w.scores = w.before + up((size_t)(batch + 2) * 8);
   w.total = w.scores + (weights ? up(rows * (size_t)w.pitch * 4) : 0);
   return w;
 }
 
-template <typename T, int HD>
-int launch_ranges(const RangeParams& p, int64_t blocks, cudaStream_t stream) {
-  using L = RangeSmem<HD>;
-  auto kern = range_kernel<T, HD>;
+template <typename T, int HD, int NR>
+int launch_line(const LineParams& p, int blocks, cudaStream_t stream) {
+  using L = LineShape<HD, NR>;
+  auto kern = line_kernel<T, HD, NR>;
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   TTJ_CUDA_TRY(cudaGetDevice(&dev));
@@ -497,28 +727,35 @@ int launch_ranges(const RangeParams& p, int64_t blocks, cudaStream_t stream) {
   return TTJ_OK;
 }
 
+template <typename T, int NR>
+int dispatch_line(const LineParams& p, int blocks, cudaStream_t stream) {
+  if (p.hd <= 64) return launch_line<T, 64, NR>(p, blocks, stream);
+  if (p.hd <= 128) return launch_line<T, 128, NR>(p, blocks, stream);
+  return launch_line<T, 256, NR>(p, blocks, stream);
+}
+
 template <typename T>
 int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   const Cuts c = cuts_of(a.batch, a.prefix_len, a.capacity, a.num_heads, a.num_kv_heads, a.head_dim);
   const bool weights = a.key_weights != nullptr && a.capacity > 0;
   const Workspace w = workspace_of(c, a.batch, a.capacity, a.num_heads, a.head_dim, a.key_weights != nullptr);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  float* part_o = reinterpret_cast<float*>(ws + w.part_o);
-  float* part_lse = reinterpret_cast<float*>(ws + w.part_lse);
-  float* scores = weights ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  float* tile_o = reinterpret_cast<float*>(ws + w.tile_o);
+  float* tile_lse = reinterpret_cast<float*>(ws + w.tile_lse);
   const int64_t group = a.num_heads / a.num_kv_heads;
   if (c.prefix_tiles)
-    if (int rc = launch_prefix_parts(a, part_o, part_lse, c.prefix_parts, c.prefix_keys, stream)) return rc;
-  RangeParams p{};
+    if (int rc = launch_prefix_parts(a, tile_o, tile_lse, c.tile_parts, c.tile_keys, stream)) return rc;
+  LineParams p{};
   p.q = a.q;
   p.pk = a.prefix_k;
   p.pv = a.prefix_v;
   p.kc = a.k_cache;
   p.vc = a.v_cache;
   p.lengths = a.lengths;
-  p.part_o = part_o;
-  p.part_lse = part_lse;
-  p.scores = scores;
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
+  p.before = reinterpret_cast<int64_t*>(ws + w.before);
+  p.scores = weights ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.q_seq = a.q_seq_stride;
   p.q_head = a.q_head_stride;
   p.pk_row = a.prefix_k_row_stride;
@@ -536,43 +773,52 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   p.prefix = (int)a.prefix_len;
   p.capacity = (int)a.capacity;
   p.num_heads = (int)a.num_heads;
-  p.kv_heads = (int)a.num_kv_heads;
+  p.heads = c.heads;
+  p.head_groups = (int)a.num_kv_heads / c.heads;
   p.group = (int)group;
   p.hd = (int)a.head_dim;
-  p.prefix_row_tiles = (int)ceil_div(a.batch * group, kRows);
-  p.prefix_keys = c.prefix_keys;
-  p.prefix_parts = c.prefix_parts;
-  p.prefix_blocks = c.prefix_tiles ? 0 : (int)(c.prefix_parts * a.num_kv_heads * p.prefix_row_tiles);
-  p.cache_row_tiles = (int)ceil_div(group, kRows);
-  p.cache_keys = c.cache_keys;
+  p.prefix_row_tiles = c.prefix_row_tiles;
+  p.prefix_units = p.head_groups * c.prefix_row_tiles;
+  p.prefix_steps = c.prefix_row_tiles > 0 ? (int)ceil_div(a.prefix_len, kStepKeys) : 0;
+  p.cache_row_tiles = c.cache_row_tiles;
+  p.pitch = c.pitch;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
-  const int64_t blocks = p.prefix_blocks + (int64_t)c.cache_parts * a.batch * a.num_kv_heads * p.cache_row_tiles;
-  if (blocks >= (int64_t)1 << 31) return fail(TTJ_ERR_UNSUPPORTED, "too many attention work items");
-  if (blocks > 0) {
-    int rc = a.head_dim <= 64    ? launch_ranges<T, 64>(p, blocks, stream)
-             : a.head_dim <= 128 ? launch_ranges<T, 128>(p, blocks, stream)
-                                 : launch_ranges<T, 256>(p, blocks, stream);
-    if (rc) return rc;
-  }
+  // Without any cached or prefix key the line is empty, but the join reads `before`.
+  const int blocks = std::max(c.blocks, 1);
+  if (int rc = c.tile_rows == 8 ? dispatch_line<T, 1>(p, blocks, stream) : dispatch_line<T, 2>(p, blocks, stream))
+    return rc;
   JoinParams j{};
-  j.part_o = part_o;
-  j.part_lse = part_lse;
-  j.scores = scores;
+  j.tile_o = tile_o;
+  j.tile_lse = tile_lse;
+  j.part_o = p.part_o;
+  j.part_lse = p.part_lse;
+  j.before = p.before;
+  j.scores = p.scores;
   j.key_weights = a.key_weights;
   j.key_weights_out = a.key_weights_out;
   j.out = a.out;
   j.lengths = a.lengths;
   j.score_pitch = w.pitch;
-  j.batch = p.batch;
+  j.rows = a.batch * a.num_heads;
+  j.out_blocks = ceil_div(j.rows, kJoinThreads / 32);
+  j.spans = weights ? (int)ceil_div(a.capacity, kWeightSpan) : 0;
   j.capacity = p.capacity;
+  j.batch = p.batch;
   j.num_heads = p.num_heads;
-  j.kv_heads = p.kv_heads;
+  j.kv_heads = (int)a.num_kv_heads;
   j.group = p.group;
   j.hd = p.hd;
-  j.parts = c.parts();
-  const dim3 grid((unsigned)(a.batch * a.num_kv_heads), weights ? (unsigned)ceil_div(a.capacity, kWeightSpan) : 1u);
-  if (grid.y > 65535u) return fail(TTJ_ERR_UNSUPPORTED, "capacity above what key_weights supports");
-  TTJ_CUDA_TRY(launch_pdl(join_kernel<T>, grid, dim3(kJoinThreads), 0, stream, j));
+  j.tile_parts = c.tile_parts;
+  j.heads_shift = c.heads == 4 ? 2 : c.heads - 1;
+  j.prefix_units = p.prefix_units;
+  j.prefix_row_tiles = p.prefix_row_tiles;
+  j.cache_row_tiles = p.cache_row_tiles;
+  j.prefix_steps = p.prefix_steps;
+  j.pitch = p.pitch;
+  j.tile_rows = c.tile_rows;
+  const int64_t grid = j.out_blocks + a.batch * a.num_kv_heads * j.spans;
+  if (grid >= (int64_t)1 << 31) return fail(TTJ_ERR_UNSUPPORTED, "batch x capacity above what one call supports");
+  TTJ_CUDA_TRY(launch_pdl(join_kernel<T>, dim3((unsigned)grid), dim3(kJoinThreads), 0, stream, j));
   return TTJ_OK;
 }
 

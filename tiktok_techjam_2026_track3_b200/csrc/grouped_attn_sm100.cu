@@ -162,21 +162,22 @@ __device__ __forceinline__ int row_limit(int r, int t, const Seg& s, const Group
   return PREFIX ? s.nk - 1 : s.rel + t * p.positions + r / p.group;
 }
 
-// Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled)
-// of tile rows r0 .. to the output rows they belong to, 16 bytes per lane.
+// Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled) to
+// the output rows they belong to, 16 bytes per lane; `at` is the output row of the
+// box's row lane % ROWS (a division each, so it is formed once per item and lane).
 template <typename T, int ROWS>
-__device__ __forceinline__ void store_box(uint32_t box, int r0, int t, int col0, const Seg& s, const GroupedParams& p) {
+__device__ __forceinline__ void store_box(uint32_t box, int64_t at, int col0, const GroupedParams& p) {
   const int lane = threadIdx.x & 31;
   const int col = col0 + 8 * (lane & 7);
 #pragma unroll
   for (int i = 0; i < ROWS; i += 4) {
     const int row = i + (lane >> 3);
-    const int64_t at = row_index(r0 + row, t, s, p);
+    const int64_t to = __shfl_sync(0xffffffffu, at, row);
     uint4 w;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                  : "r"(box + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) : "memory");
-    if (at >= 0 && col < p.hd) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.hd + col) = w;
+    if (to >= 0 && col < p.hd) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to * p.hd + col) = w;
   }
 }
 
@@ -353,7 +354,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
         st_shared_u32(box + (g + 8) * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wb);
       }
       __syncwarp();
-      store_box<T, 16>(box, r0, t, 0, s, p);
+      store_box<T, 16>(box, row_index(r0 + (lane & 15), t, s, p), 0, p);
       __syncwarp();  // the box is written again at the next item's end
     }
     // The next item's first P.V overwrites O_t only after this thread's next
@@ -507,7 +508,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
           }
         }
         __syncwarp();
-        store_box<T, 32>(box, r0, t, 64 * hh, sg, p);
+        store_box<T, 32>(box, at, 64 * hh, p);
         __syncwarp();
       }
     }

@@ -405,24 +405,44 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 # ------------------------------------------------------- serving: prompts, caches
 
-def _strided(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, Tuple[int, ...]]:
-    """(t, element strides of all dimensions but the last): views whose rows are
-    contiguous and 16-byte aligned are read in place, anything else is copied."""
+def _strided(t: torch.Tensor, name: str) -> Tuple:
+    """(t, address, element strides of all dimensions but the last): views whose rows
+    are contiguous and 16-byte aligned are read in place, anything else is copied."""
+    st, p = t.stride(), t.data_ptr()
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor (got {t.device}); there is no CPU path")
-    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
-    if (t.stride(-1) != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s <= 0 or s % 8 for _, s in lead):
+    if len(st) == 3:
+        a, b, c = st
+        if c == 1 and a > 0 and b > 0 and not (a | b) & 7 and not p & 15:
+            return t, p, a, b
+    else:
+        a, b, c, d = st
+        if d == 1 and a > 0 and b > 0 and c > 0 and not (a | b | c) & 7 and not p & 15:
+            return t, p, a, b, c
+    lead = [s for n, s in zip(t.shape[:-1], st[:-1]) if n > 1]
+    if st[-1] != 1 or p % 16 or any(s <= 0 or s % 8 for s in lead):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
     # a dimension of one element has no stride of its own; give it a valid one
-    return t, tuple(s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    return (t, t.data_ptr(), *(s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1])))
 
 
 def _same(ref: torch.Tensor, **tensors: torch.Tensor) -> None:
+    dtype, device = ref.dtype, ref.device
     for name, t in tensors.items():
-        if t.dtype != ref.dtype or t.device != ref.device:
-            raise RuntimeError(f"{name} must be {ref.dtype} on {ref.device}, got {t.dtype} on {t.device}")
+        if t.dtype != dtype or t.device != device:
+            raise RuntimeError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+
+
+def _launch(call: _lib.PackedCall, device: torch.device, *values) -> None:
+    """Enqueue on `device`'s current stream, with that device current."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        call(torch._C._cuda_getCurrentRawStream(index), *values)
+    else:
+        with torch.cuda.device(device):
+            call(torch._C._cuda_getCurrentRawStream(index), *values)
 
 
 def _group(num_heads: int, num_kv_heads: int) -> int:
@@ -453,6 +473,8 @@ class PromptPlan:
                                              C.cast(host.data_ptr(), C.POINTER(C.c_int32)), n),
                    "ttj_prompt_plan_build")
         self.entries = int(n)
+        self.q_shape = torch.Size((self.tokens, num_heads, head_dim))
+        self.kv_shape = torch.Size((self.tokens, num_kv_heads, head_dim))
         self.table = host.to(device)
 
     @property
@@ -468,48 +490,34 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PromptP
     h // (Hq / Hkv).  Returns [T,Hq,hd], and with ``return_lse`` also the log of
     each row's sum of exponentials, fp32 [T,Hq].  Views with strided rows (slices
     of a packed projection) are read in place.  scale defaults to hd ** -0.5."""
-    lib = _lib.load()
     dt = _dtype_code(q)
-    want_q = (plan.tokens, plan.num_heads, plan.head_dim)
-    want_kv = (plan.tokens, plan.num_kv_heads, plan.head_dim)
-    for t, n, want in ((q, "q", want_q), (k, "k", want_kv), (v, "v", want_kv)):
-        if tuple(t.shape) != want:
-            raise RuntimeError(f"{n} must be {list(want)} for this plan, got {list(t.shape)}")
+    if q.shape != plan.q_shape or k.shape != plan.kv_shape or v.shape != plan.kv_shape:
+        for t, n, want in ((q, "q", plan.q_shape), (k, "k", plan.kv_shape), (v, "v", plan.kv_shape)):
+            if t.shape != want:
+                raise RuntimeError(f"{n} must be {list(want)} for this plan, got {list(t.shape)}")
     _same(q, k=k, v=v)
-    q, qs = _strided(q, "q")
-    k, ks = _strided(k, "k")
-    v, vs = _strided(v, "v")
-    if plan.device != q.device:
-        raise RuntimeError(f"the plan is on {plan.device}, q on {q.device}")
+    q, qp, qt, qh = _strided(q, "q")
+    k, kp, kt, kh = _strided(k, "k")
+    v, vp, vt, vh = _strided(v, "v")
+    dev = q.device
+    if plan.table.device != dev:
+        raise RuntimeError(f"the plan is on {plan.device}, q on {dev}")
     if out is None:
-        out = torch.empty(want_q, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != want_q or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        out = q.new_empty(plan.q_shape)
+    elif out.shape != plan.q_shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [T,Hq,hd] tensor of q's dtype on q's device")
-    lse = torch.empty(want_q[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    a = _lib.PromptAttnArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=_ptr(lse),
-        plan=plan.table.data_ptr(), plan_entries=plan.entries, status=status_word(q.device).data_ptr(),
-        tokens=plan.tokens, num_heads=plan.num_heads, num_kv_heads=plan.num_kv_heads, head_dim=plan.head_dim,
-        q_token_stride=qs[0], q_head_stride=qs[1], k_token_stride=ks[0], k_head_stride=ks[1],
-        v_token_stride=vs[0], v_head_stride=vs[1],
-        scale=plan.head_dim ** -0.5 if scale is None else float(scale), dtype=dt)
-    with torch.cuda.device(q.device):
-        _lib.check(lib.ttj_prompt_attn_fwd(C.byref(a), _stream(q.device)), "ttj_prompt_attn_fwd")
+    lse = torch.empty(plan.q_shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    _launch(_lib.prompt_attn_fwd, dev, qp, kp, vp, out.data_ptr(), _ptr(lse) or 0, plan.table.data_ptr(),
+            plan.entries, status_word(dev).data_ptr(), plan.tokens, plan.num_heads, plan.num_kv_heads,
+            plan.head_dim, qt, qh, kt, kh, vt, vh, plan.head_dim ** -0.5 if scale is None else float(scale), dt)
     return (out, lse) if return_lse else out
 
 
-def _lengths(lengths: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
-    if tuple(lengths.shape) != (batch,) or lengths.dtype != torch.int32 or lengths.device != device:
-        raise RuntimeError(f"lengths must be int32 [{batch}] on {device}, got {lengths.dtype} "
-                           f"{list(lengths.shape)} on {lengths.device}")
-    return lengths.contiguous()
-
-
-def _key_weights(w: torch.Tensor, shape: Tuple[int, ...], device: torch.device) -> torch.Tensor:
-    if tuple(w.shape) != shape or w.dtype != torch.float32 or w.device != device:
-        raise RuntimeError(f"key_weights must be float32 {list(shape)} on {device}, got {w.dtype} "
-                           f"{list(w.shape)} on {w.device}")
-    return w.contiguous()
+def _dense(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"{name} must be {str(dtype)[6:]} {list(shape)} on {device}, got {str(t.dtype)[6:]} "
+                           f"{list(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -524,51 +532,42 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     With ``key_weights`` (fp32 [B,Hkv,C]) it returns (out, new_key_weights): each
     cached key's weight plus this step's probabilities of that key summed over
     the group's heads, for ``cache_evict``; the input is not written."""
-    lib = _lib.load()
     dt = _dtype_code(q)
     if q.dim() != 3 or prefix_k.dim() != 3 or k_cache.dim() != 4:
         raise RuntimeError("q must be [B,Hq,hd], prefix_k and prefix_v [P,Hkv,hd], k_cache and v_cache [B,C,Hkv,hd]")
     B, Hq, hd = q.shape
-    P, Hkv = prefix_k.shape[:2]
+    P, Hkv, _ = prefix_k.shape
     Cap = k_cache.shape[1]
     _group(Hq, Hkv)
-    for t, n, want in ((prefix_k, "prefix_k", (P, Hkv, hd)), (prefix_v, "prefix_v", (P, Hkv, hd)),
-                       (k_cache, "k_cache", (B, Cap, Hkv, hd)), (v_cache, "v_cache", (B, Cap, Hkv, hd))):
-        if tuple(t.shape) != want:
-            raise RuntimeError(f"{n} must be {list(want)}, got {list(t.shape)}")
+    shared, own = (P, Hkv, hd), (B, Cap, Hkv, hd)
+    if prefix_k.shape != shared or prefix_v.shape != shared or k_cache.shape != own or v_cache.shape != own:
+        for t, n, want in ((prefix_k, "prefix_k", shared), (prefix_v, "prefix_v", shared),
+                           (k_cache, "k_cache", own), (v_cache, "v_cache", own)):
+            if t.shape != want:
+                raise RuntimeError(f"{n} must be {list(want)}, got {list(t.shape)}")
     _same(q, prefix_k=prefix_k, prefix_v=prefix_v, k_cache=k_cache, v_cache=v_cache)
-    q, qs = _strided(q, "q")
-    prefix_k, pks = _strided(prefix_k, "prefix_k")
-    prefix_v, pvs = _strided(prefix_v, "prefix_v")
-    k_cache, kcs = _strided(k_cache, "k_cache")
-    v_cache, vcs = _strided(v_cache, "v_cache")
-    lengths = _lengths(lengths, B, q.device)
+    q, qp, qs, qh = _strided(q, "q")
+    prefix_k, pkp, pkr, pkh = _strided(prefix_k, "prefix_k")
+    prefix_v, pvp, pvr, pvh = _strided(prefix_v, "prefix_v")
+    k_cache, kp, ks, kr, kh = _strided(k_cache, "k_cache")
+    v_cache, vp, vs, vr, vh = _strided(v_cache, "v_cache")
+    dev = q.device
+    lengths = _dense(lengths, "lengths", (B,), torch.int32, dev)
     new_weights = None
     if key_weights is not None:
-        key_weights = _key_weights(key_weights, (B, Hkv, Cap), q.device)
+        key_weights = _dense(key_weights, "key_weights", (B, Hkv, Cap), torch.float32, dev)
         new_weights = torch.empty_like(key_weights)
     if out is None:
-        out = torch.empty(B, Hq, hd, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != (B, Hq, hd) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        out = q.new_empty((B, Hq, hd))
+    elif out.shape != (B, Hq, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
-    with torch.cuda.device(q.device):
-        need = lib.ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, int(key_weights is not None))
+    need = _lib.load().ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, key_weights is not None)
     if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    a = _lib.SharedPrefixAttnArgs(
-        q=q.data_ptr(), prefix_k=prefix_k.data_ptr(), prefix_v=prefix_v.data_ptr(),
-        k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), lengths=lengths.data_ptr(),
-        key_weights=_ptr(key_weights), key_weights_out=_ptr(new_weights), out=out.data_ptr(),
-        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(), status=status_word(q.device).data_ptr(),
-        batch=B, prefix_len=P, capacity=Cap, num_heads=Hq, num_kv_heads=Hkv, head_dim=hd,
-        q_seq_stride=qs[0], q_head_stride=qs[1],
-        prefix_k_row_stride=pks[0], prefix_k_head_stride=pks[1],
-        prefix_v_row_stride=pvs[0], prefix_v_head_stride=pvs[1],
-        k_seq_stride=kcs[0], k_row_stride=kcs[1], k_head_stride=kcs[2],
-        v_seq_stride=vcs[0], v_row_stride=vcs[1], v_head_stride=vcs[2],
-        scale=hd ** -0.5 if scale is None else float(scale), dtype=dt)
-    with torch.cuda.device(q.device):
-        _lib.check(lib.ttj_shared_prefix_attn_fwd(C.byref(a), _stream(q.device)), "ttj_shared_prefix_attn_fwd")
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch(_lib.shared_prefix_attn_fwd, dev, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
+            _ptr(new_weights) or 0, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+            status_word(dev).data_ptr(), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
+            hd ** -0.5 if scale is None else float(scale), dt)
     return out if new_weights is None else (out, new_weights)
 
 
@@ -592,7 +591,6 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
     zeros.  ``out`` = (k, v) of at least ``budget`` rows takes the result in place
     of fresh caches (rows from ``budget`` on are left alone); it must not alias
     the input."""
-    lib = _lib.load()
     _dtype_code(k_cache)
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise RuntimeError(f"k_cache and v_cache must both be [B,C,Hkv,hd], got {list(k_cache.shape)} and {list(v_cache.shape)}")
@@ -602,34 +600,27 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
         raise RuntimeError(f"budget must be positive and recent in 0 .. budget, got {budget} and {recent}")
     _same(k_cache, v_cache=v_cache)
     dev = k_cache.device
-    k_cache, kcs = _strided(k_cache, "k_cache")
-    v_cache, vcs = _strided(v_cache, "v_cache")
-    lengths = _lengths(lengths, B, dev)
-    key_weights = _key_weights(key_weights, (B, Hkv, Cap), dev)
+    k_cache, kp, ks, kr, kh = _strided(k_cache, "k_cache")
+    v_cache, vp, vs, vr, vh = _strided(v_cache, "v_cache")
+    lengths = _dense(lengths, "lengths", (B,), torch.int32, dev)
+    key_weights = _dense(key_weights, "key_weights", (B, Hkv, Cap), torch.float32, dev)
     if out is None:
-        k_out = torch.empty(B, budget, Hkv, hd, dtype=k_cache.dtype, device=dev)
-        v_out = torch.empty_like(k_out)
+        k_out = k_cache.new_empty((B, budget, Hkv, hd))
+        v_out = k_cache.new_empty((B, budget, Hkv, hd))
     else:
         k_out, v_out = out
         _same(k_cache, k_out=k_out, v_out=v_out)
         for t, n in ((k_out, "k_out"), (v_out, "v_out")):
-            if t.dim() != 4 or t.shape[0] != B or t.shape[1] < budget or tuple(t.shape[2:]) != (Hkv, hd):
+            if t.dim() != 4 or t.shape[0] != B or t.shape[1] < budget or t.shape[2:] != (Hkv, hd):
                 raise RuntimeError(f"{n} must be [{B}, >={budget}, {Hkv}, {hd}], got {list(t.shape)}")
-    (ko, kos), (vo, vos) = _strided(k_out, "k_out"), _strided(v_out, "v_out")
+    ko, kop, kos, kor, koh = _strided(k_out, "k_out")
+    vo, vop, vos, vor, voh = _strided(v_out, "v_out")
     if ko is not k_out or vo is not v_out:
         raise RuntimeError("out must have contiguous rows and 16-byte aligned strides")
-    weights = torch.empty(B, Hkv, budget, dtype=torch.float32, device=dev)
-    new_lengths = torch.empty(B, dtype=torch.int32, device=dev)
-    positions = torch.empty(B, Hkv, budget, dtype=torch.int32, device=dev)
-    a = _lib.CacheEvictArgs(
-        k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), key_weights=key_weights.data_ptr(),
-        lengths=lengths.data_ptr(), k_out=k_out.data_ptr(), v_out=v_out.data_ptr(),
-        weights_out=weights.data_ptr(), lengths_out=new_lengths.data_ptr(), positions_out=positions.data_ptr(),
-        batch=B, capacity=Cap, num_kv_heads=Hkv, head_dim=hd, budget=budget, recent=recent,
-        k_seq_stride=kcs[0], k_row_stride=kcs[1], k_head_stride=kcs[2],
-        v_seq_stride=vcs[0], v_row_stride=vcs[1], v_head_stride=vcs[2],
-        k_out_seq_stride=kos[0], k_out_row_stride=kos[1], k_out_head_stride=kos[2],
-        v_out_seq_stride=vos[0], v_out_row_stride=vos[1], v_out_head_stride=vos[2])
-    with torch.cuda.device(dev):
-        _lib.check(lib.ttj_cache_evict(C.byref(a), _stream(dev)), "ttj_cache_evict")
+    weights = key_weights.new_empty((B, Hkv, budget))
+    new_lengths = lengths.new_empty((B,))
+    positions = lengths.new_empty((B, Hkv, budget))
+    _launch(_lib.cache_evict, dev, kp, vp, key_weights.data_ptr(), lengths.data_ptr(), kop, vop, weights.data_ptr(),
+            new_lengths.data_ptr(), positions.data_ptr(), B, Cap, Hkv, hd, budget, recent, ks, kr, kh, vs, vr, vh,
+            kos, kor, koh, vos, vor, voh)
     return EvictedCache(k_out, v_out, weights, new_lengths, positions)
