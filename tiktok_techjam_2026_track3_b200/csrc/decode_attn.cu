@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kJoinThreads = 256;
-constexpr int kWeightSpan = 1024;  // cached keys per join block
+constexpr int kWeightStep = 1024;  // cached keys per join block and step
 constexpr int kMinSteps = 2;       // of a stretch
 
 // NR: row tiles of 8 (group heads) that a warp carries, 1 or 2.
@@ -78,6 +78,7 @@ struct LineParams {
   int64_t score_pitch;
   int batch, prefix, capacity, num_heads, head_groups, heads, group, hd;  // kv heads = head_groups * heads
   int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch;
+  int after_prefix;         // launched behind the prefix kernel of the same step
   float scale_log2;
 };
 
@@ -147,7 +148,10 @@ line_kernel(const LineParams p) {
   constexpr int kRows = 8 * NR;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_before[kWarps * 32 + 1];  // steps before each thread's sequences, and of all
-  grid_dependency_wait();
+  // Behind the prefix kernel of the same step nothing of that kernel is read, and it
+  // has let this one start only once everything before it was complete: the wait
+  // moves to the end, where it keeps the join behind both.
+  if (!p.after_prefix) grid_dependency_wait();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, kq = lane & 3;
@@ -198,7 +202,10 @@ line_kernel(const LineParams p) {
   const int64_t stretch = stretch_of(total, gridDim.x * kWarps / p.heads);
   const int64_t from = worker * stretch;
   const int steps = (int)min(stretch, total - from);
-  if (steps <= 0) return;  // uniform over the warp; no block barrier follows
+  if (steps <= 0) {  // uniform over the warp; no block barrier follows
+    if (p.after_prefix) grid_dependency_wait();
+    return;
+  }
 
   Place at;
   if (from < prefix_total) {
@@ -457,6 +464,7 @@ line_kernel(const LineParams p) {
     }
     if (i + 1 < steps) advance(at);
   }
+  if (p.after_prefix) grid_dependency_wait();
 }
 
 struct JoinParams {
@@ -468,7 +476,7 @@ struct JoinParams {
   void* out;
   const int32_t* lengths;
   int64_t score_pitch, rows, out_blocks;
-  int spans;                           // of kWeightSpan cached keys
+  int spans, span;                     // spans of `span` cached keys
   int capacity, batch, num_heads, kv_heads, group, hd, tile_parts;
   int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch, tile_rows;
   int heads_shift;                     // log2 of the line's heads
@@ -603,56 +611,60 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
     return;
   }
   __shared__ float s_lse[kMaxGroup];
-  int64_t rest = blockIdx.x - p.out_blocks;
-  const int64_t bh = rest / p.spans;
-  const int span = (int)(rest - bh * p.spans);
-  const int64_t b = bh / p.kv_heads;
+  const int64_t rest = blockIdx.x - p.out_blocks;
+  const int64_t bh = div_of(rest, p.spans);
+  const int64_t b = div_of(bh, p.kv_heads);
   const int kvh = (int)(bh - b * p.kv_heads);
   const int n = min(max(__ldg(p.lengths + b), 0), p.capacity);
-  const int c0 = span * kWeightSpan + threadIdx.x;
-  constexpr int kPer = kWeightSpan / kJoinThreads;
-  float sum[kPer], w[kPer];
+  const int from = (int)(rest - bh * p.spans) * p.span, to = (int)min((int64_t)from + p.span, (int64_t)p.capacity);
+  constexpr int kPer = kWeightStep / kJoinThreads;
+  constexpr int kAhead = 4;      // rows whose scores are read together
+  const float* scores = p.scores + (b * p.num_heads + kvh * p.group) * p.score_pitch;
+  float x[kAhead][kPer];
+  auto fetch = [&](int c0, int r0) {
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    const int c = c0 + q * kJoinThreads;
-    sum[q] = 0.f;
-    w[q] = c < p.capacity ? __ldg(p.key_weights + bh * p.capacity + c) : 0.f;
-  }
-  if (span * kWeightSpan < n) {  // uniform
-    const float* scores = p.scores + (b * p.num_heads + kvh * p.group) * p.score_pitch;
-    constexpr int kAhead = 4;    // rows whose scores are read before the lse are known
-    float x[kAhead][kPer];
-    auto fetch = [&](int r0) {
+    for (int r = 0; r < kAhead; ++r)
 #pragma unroll
-      for (int r = 0; r < kAhead; ++r)
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-          const int c = c0 + q * kJoinThreads;
-          x[r][q] = r0 + r < p.group && c < n ? __ldg(scores + (r0 + r) * p.score_pitch + c) : -INFINITY;
-        }
-    };
-    fetch(0);
+      for (int q = 0; q < kPer; ++q) {
+        const int c = c0 + q * kJoinThreads;
+        x[r][q] = r0 + r < p.group && c < min(n, to) ? __ldg(scores + (r0 + r) * p.score_pitch + c) : -INFINITY;
+      }
+  };
+  fetch(from + threadIdx.x, 0);  // before the lse are known
+  if (from < n) {                // uniform
     for (int r = warp; r < p.group; r += kJoinThreads / 32) {
       const RowParts y = row_parts(p, b, kvh * p.group + r);
       const float lse = row_lse(p, y, p.tile_parts + y.prefix_count + y.cache_count);
       if (lane == 0) s_lse[r] = lse;
     }
     __syncthreads();
-    for (int r0 = 0; r0 < p.group; r0 += kAhead) {
-      if (r0 > 0) fetch(r0);
-#pragma unroll
-      for (int r = 0; r < kAhead; ++r)
-        if (r0 + r < p.group) {
-          const float lse = s_lse[r0 + r];
-#pragma unroll
-          for (int q = 0; q < kPer; ++q) sum[q] += fast_exp2(x[r][q] - lse);
-        }
-    }
   }
+  for (int c0 = from + threadIdx.x; c0 - (int)threadIdx.x < to; c0 += kWeightStep) {
+    float w[kPer], sum[kPer];
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) {
-    const int c = c0 + q * kJoinThreads;
-    if (c < p.capacity) p.key_weights_out[bh * p.capacity + c] = w[q] + (c < n ? sum[q] : 0.f);
+    for (int q = 0; q < kPer; ++q) {
+      const int c = c0 + q * kJoinThreads;
+      w[q] = c < to ? __ldg(p.key_weights + bh * p.capacity + c) : 0.f;
+      sum[q] = 0.f;
+    }
+    if (c0 - (int)threadIdx.x < n) {
+      if (c0 != from + (int)threadIdx.x) fetch(c0, 0);
+      for (int r0 = 0; r0 < p.group; r0 += kAhead) {
+        if (r0 > 0) fetch(c0, r0);
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r)
+          if (r0 + r < p.group) {
+            const float lse = s_lse[r0 + r];
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) sum[q] += fast_exp2(x[r][q] - lse);
+          }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int c = c0 + q * kJoinThreads;
+      if (c < to) p.key_weights_out[bh * p.capacity + c] = w[q] + (c < n ? sum[q] : 0.f);
+    }
   }
 }
 
@@ -782,6 +794,7 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   p.prefix_steps = c.prefix_row_tiles > 0 ? (int)ceil_div(a.prefix_len, kStepKeys) : 0;
   p.cache_row_tiles = c.cache_row_tiles;
   p.pitch = c.pitch;
+  p.after_prefix = c.prefix_tiles;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   // Without any cached or prefix key the line is empty, but the join reads `before`.
   const int blocks = std::max(c.blocks, 1);
@@ -801,7 +814,12 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   j.score_pitch = w.pitch;
   j.rows = a.batch * a.num_heads;
   j.out_blocks = ceil_div(j.rows, kJoinThreads / 32);
-  j.spans = weights ? (int)ceil_div(a.capacity, kWeightSpan) : 0;
+  // A block's start (its rows' lse) costs about two steps: only as many spans as fill
+  // the GPU about three times.
+  const int64_t steps = ceil_div(a.capacity, kWeightStep);
+  const int64_t wanted = ceil_div(9 * (int64_t)sm_count(), a.batch * a.num_kv_heads);
+  j.span = (int)(ceil_div(steps, std::max<int64_t>(1, std::min(steps, wanted))) * kWeightStep);
+  j.spans = weights ? (int)ceil_div(a.capacity, j.span) : 0;
   j.capacity = p.capacity;
   j.batch = p.batch;
   j.num_heads = p.num_heads;
