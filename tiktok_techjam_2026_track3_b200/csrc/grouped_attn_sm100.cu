@@ -59,6 +59,8 @@ struct GroupedParams {
   int num_items, num_entries, kv_heads, group, positions;  // positions = 128 / group
   int num_heads, hd;
   int head_major;         // item order: 1 = a head's entries consecutive
+  int kv_shift;           // log2 of kv_heads, or -1
+  int box_store;          // a softmax warp's rows are whole groups: its output rows form a TMA box
   int batch, prefix, split_keys, row_items;  // prefix: row_items = ceil(B / (tiles * positions))
   float scale_log2;
   int* status;
@@ -116,7 +118,7 @@ __device__ __forceinline__ Seg seg_of(int item, const GroupedParams& p) {
       s.kvh = item / p.num_entries;
       e = item - s.kvh * p.num_entries;
     } else {
-      e = item / p.kv_heads;
+      e = p.kv_shift >= 0 ? item >> p.kv_shift : item / p.kv_heads;
       s.kvh = item - e * p.kv_heads;
     }
     const int4 w = __ldg(p.plan + e);
@@ -147,27 +149,42 @@ __device__ __forceinline__ int item_tiles(const Seg& s, int positions) {
   return NT == 2 ? max(a, key_tiles(tile_keys<PREFIX>(s, 1, positions))) : a;
 }
 
-// Where row r of a tile (r = position * group + head) goes: its row index in
-// [tokens][Hq] (or [sequences][Hq]), or -1 for a row that is no position's.
-__device__ __forceinline__ int64_t row_index(int r, int t, const Seg& s, const GroupedParams& p) {
-  const int pos = r / p.group;
+// Row r of a tile is position r / group, head r % group; the positions of the rows a
+// thread deals with are formed once (row_pos), not per item.
+__device__ __forceinline__ int row_pos(int r, const GroupedParams& p) { return r / p.group; }
+
+// Where row r = (pos, head r - pos * group) of tile t goes: its row in [tokens][Hq]
+// (or [sequences][Hq]), or -1 for a row that is no position's.
+__device__ __forceinline__ int64_t row_index(int r, int pos, int t, const Seg& s, const GroupedParams& p) {
   const int at = t * p.positions + pos;
   if (pos >= p.positions || at >= s.nq) return -1;
   return (int64_t)(s.q0 + at) * p.num_heads + s.kvh * p.group + (r - pos * p.group);
 }
 
-// Last key (relative to the item's first) that row r of tile t sees.
+// Last key (relative to the item's first) that position pos of tile t sees.
 template <bool PREFIX>
-__device__ __forceinline__ int row_limit(int r, int t, const Seg& s, const GroupedParams& p) {
-  return PREFIX ? s.nk - 1 : s.rel + t * p.positions + r / p.group;
+__device__ __forceinline__ int row_limit(int pos, int t, const Seg& s, const GroupedParams& p) {
+  return PREFIX ? s.nk - 1 : s.rel + t * p.positions + pos;
 }
 
-// Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled) to
-// the output rows they belong to, 16 bytes per lane; `at` is the output row of the
-// box's row lane % ROWS (a division each, so it is formed once per item and lane).
+// Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled): as
+// one TMA box where all its rows are positions of this prompt, else row by row, 16
+// bytes per lane, `at` being the output row of the box's row lane % ROWS.  (The row
+// by row form kept a warp ~1500 cycles per box, with its 8 dependent stores.)
 template <typename T, int ROWS>
-__device__ __forceinline__ void store_box(uint32_t box, int64_t at, int col0, const GroupedParams& p) {
+__device__ __forceinline__ void store_box(uint32_t box, int64_t at, int r0, int t, int col0, const Seg& s,
+                                          const CUtensorMap* tm_out, const GroupedParams& p) {
   const int lane = threadIdx.x & 31;
+  if (p.box_store && __all_sync(0xffffffffu, at >= 0)) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_4d(tm_out, box, col0, 0, s.kvh, s.q0 + t * p.positions + row_pos(r0, p));
+      bulk_commit_group();
+    }
+    return;
+  }
+  __syncwarp();
   const int col = col0 + 8 * (lane & 7);
 #pragma unroll
   for (int i = 0; i < ROWS; i += 4) {
@@ -180,12 +197,18 @@ __device__ __forceinline__ void store_box(uint32_t box, int64_t at, int col0, co
     if (to >= 0 && col < p.hd) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to * p.hd + col) = w;
   }
 }
+// Before a box is written again: its last store has read it.
+__device__ __forceinline__ void box_free() {
+  if ((threadIdx.x & 31) == 0) bulk_wait_group_read<0>();
+  __syncwarp();
+}
 
 // Softmax, two warps per tile and TMEM lane quarter (head_dim 64): warp w serves
 // tile (w - 4) / 8 and 16 rows; lane 4g + k holds rows g and g + 8 of them and of
 // each 8-key group n keys 8n + 2k and 8n + 2k + 1 (the 16-lane TMEM shapes).
 template <typename T, int HD, bool PREFIX>
 __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* epi_base, uint32_t tmem,
+                                              const CUtensorMap* tm_out,
                                               uint64_t* s_full, uint64_t* s_free, uint64_t* p_full,
                                               uint64_t* o_done, volatile int* abort_flag) {
   using L = GroupedSmem<HD>;
@@ -200,6 +223,9 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
   const uint32_t t_p = t_lane + L::kColP + t * 64;
   const uint32_t t_o = t_lane + L::kColO + t * HD;
   const uint32_t box = smem_u32(epi_base) + (warp - 4) * (L::kEpiRows * 128);
+  // positions of this lane's rows g, g + 8 and of the box's row lane % 16, a byte each
+  const uint32_t pos3 = (uint32_t)row_pos(r0 + g, p) | (uint32_t)row_pos(r0 + g + 8, p) << 8 |
+                        (uint32_t)row_pos(r0 + (lane & 15), p) << 16;
   uint32_t sf_phase = 0, od_phase = 0;
   auto row_max4 = [](float v) {  // over the four threads of a row
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -217,8 +243,8 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
     {
       const Seg s = seg_of<PREFIX, L::kNT>(item, p);
       n_kv = key_tiles(tile_keys<PREFIX>(s, t, p.positions));
-      lim_a = row_limit<PREFIX>(r0 + g, t, s, p) - 2 * kq;
-      lim_b = row_limit<PREFIX>(r0 + g + 8, t, s, p) - 2 * kq;
+      lim_a = row_limit<PREFIX>(pos3 & 255, t, s, p) - 2 * kq;
+      lim_b = row_limit<PREFIX>((pos3 >> 8) & 255, t, s, p) - 2 * kq;
       lim_first = row_limit<PREFIX>(0, t, s, p);
     }
     if (n_kv == 0) continue;
@@ -323,7 +349,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
     const Seg s = seg_of<PREFIX, L::kNT>(item, p);
     float* lse = PREFIX ? p.part_lse + (int64_t)s.part * p.batch * p.num_heads : p.lse;
     if (lse != nullptr && kq < 2) {  // one thread per row
-      const int64_t at = row_index(r0 + g + 8 * kq, t, s, p);
+      const int64_t at = row_index(r0 + g + 8 * kq, (pos3 >> (8 * kq)) & 255, t, s, p);
       const float v = kq == 0 ? m_a + log2f(l_a) : m_b + log2f(l_b);
       if (at >= 0) lse[at] = PREFIX ? v : v * 0.69314718055994531f;
     }
@@ -333,7 +359,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
     uint32_t o[32];  // o[4n + e]: row (e < 2 ? a : b), column 8n + 2k + (e & 1)
     tmem_ld_16x256b_x8(t_o, o);
     if constexpr (PREFIX) {
-      const int64_t ra = row_index(r0 + g, t, s, p), rb = row_index(r0 + g + 8, t, s, p);
+      const int64_t ra = row_index(r0 + g, pos3 & 255, t, s, p), rb = row_index(r0 + g + 8, (pos3 >> 8) & 255, t, s, p);
       float* part = p.part_o + (int64_t)s.part * p.batch * p.num_heads * p.hd;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -345,6 +371,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
             make_float2(__uint_as_float(o[4 * n + 2]) * inv_b, __uint_as_float(o[4 * n + 3]) * inv_b);
       }
     } else {
+      box_free();
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         // 128-byte rows, 16-byte chunk n holds columns 8n..8n+7, swizzled by row & 7
@@ -353,19 +380,19 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
         st_shared_u32(box + g * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wa);
         st_shared_u32(box + (g + 8) * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wb);
       }
-      __syncwarp();
-      store_box<T, 16>(box, row_index(r0 + (lane & 15), t, s, p), 0, p);
-      __syncwarp();  // the box is written again at the next item's end
+      store_box<T, 16>(box, row_index(r0 + (lane & 15), pos3 >> 16, t, s, p), r0, t, 0, s, tm_out, p);
     }
     // The next item's first P.V overwrites O_t only after this thread's next
     // p_full arrival, which follows these TMEM loads.
   }
+  if (lane == 0) bulk_wait_group_all();  // output boxes complete before exit
 }
 
 // Softmax, one warp per tile and TMEM lane quarter, thread = row, P over S
 // (head_dim 128 and 256).
 template <typename T, int HD, bool PREFIX>
 __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* epi_base, uint32_t tmem,
+                                             const CUtensorMap* tm_out,
                                              uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
                                              volatile int* abort_flag) {
   using L = GroupedSmem<HD>;
@@ -380,15 +407,17 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
   const uint32_t t_p = t_lane + L::kColP + t * L::kPStride;
   const uint32_t t_o = t_lane + L::kColO + t * HD;
   const uint32_t box = smem_u32(epi_base) + (warp - 4) * (L::kEpiRows * 128);
+  const int pos = row_pos(r, p);
   uint32_t sf_phase = 0, od_phase = 0;
   bool ok = true;
+  Seg next = seg_of<PREFIX, L::kNT>(item_of(0), p);  // (every block has an item)
   for (int k = 0; ok; ++k) {
-    const int item = item_of(k);
-    if (item >= p.num_items) break;
-    const Seg sg = seg_of<PREFIX, L::kNT>(item, p);
-    const int n_kv = key_tiles(tile_keys<PREFIX>(sg, t, p.positions));
+    if (item_of(k) >= p.num_items) break;
+    const Seg sg = next;
+    if (item_of(k + 1) < p.num_items) next = seg_of<PREFIX, L::kNT>(item_of(k + 1), p);
+    const int keys = tile_keys<PREFIX>(sg, t, p.positions), n_kv = key_tiles(keys);
     if (n_kv == 0) continue;
-    const int limit = row_limit<PREFIX>(r, t, sg, p), lim_first = row_limit<PREFIX>(0, t, sg, p);
+    const int limit = row_limit<PREFIX>(pos, t, sg, p), lim_first = row_limit<PREFIX>(0, t, sg, p);
     float m_run = -INFINITY;  // exponent reference (log2 units), moved lazily
     float l_run = 0.f;        // running sum of P in fp32
     for (int j = 0; j < n_kv; ++j) {
@@ -408,17 +437,22 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
 #pragma unroll
         for (int i = 0; i < kTile; ++i) s[i] = i <= lim ? s[i] : -INFINITY;
       }
-      // row max: eight independent chains of 3-input max
-      float mx8[8];
+      // Keys past the tile's last visible one are computed neither by Q.K nor read by
+      // P.V; the softmax skips them 32 at a time.
+      const int chunks = (min(keys - k0, kTile) + 31) >> 5;
+      // row max: eight independent chains of 3-input max per half
+      auto half_max = [&](int i0) {
+        float mx8[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) mx8[q] = fmax3(s[q], s[8 + q], s[16 + q]);
+        for (int q = 0; q < 8; ++q) mx8[q] = fmaxf(s[i0 + q], s[i0 + 8 + q]);
 #pragma unroll
-      for (int i = 24; i < kTile - 8; i += 16)
+        for (int i = 16; i < 64; i += 16)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], s[i + q], s[i + 8 + q]);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) mx8[q] = fmaxf(mx8[q], s[kTile - 8 + q]);
-      const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+          for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], s[i0 + i + q], s[i0 + i + 8 + q]);
+        return fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
+      };
+      float mx = half_max(0);
+      if (chunks > 2) mx = fmaxf(mx, half_max(64));
       const float m_tile = mx * p.scale_log2;
       const float m_new = (m_tile > m_run + 8.f) ? m_tile : m_run;
       const float m_use = m_new == -INFINITY ? 0.f : m_new;
@@ -429,6 +463,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
       uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < kTile / 32; ++c) {
+        if (c >= chunks) break;  // uniform
         uint32_t (&pc)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[c >> 1][(c & 1) * 16]);
 #pragma unroll
         for (int ii = 0; ii < 16; ++ii) {
@@ -462,7 +497,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
       mbar_arrive(&p_full[t]);
     }
     if (!ok) break;
-    const int64_t at = row_index(r, t, sg, p);
+    const int64_t at = row_index(r, pos, t, sg, p);
     float* lse = PREFIX ? p.part_lse + (int64_t)sg.part * p.batch * p.num_heads : p.lse;
     if (lse != nullptr && at >= 0) {
       const float v = m_run + log2f(l_run);
@@ -492,6 +527,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
 #pragma unroll 1
       for (int hh = 0; hh < HD / 64; ++hh) {
         if (64 * hh >= p.hd) break;  // only zero padding left (uniform)
+        box_free();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t o[32];
@@ -507,18 +543,18 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
                          "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
           }
         }
-        __syncwarp();
-        store_box<T, 32>(box, at, 64 * hh, p);
-        __syncwarp();
+        store_box<T, 32>(box, at, r0, t, 64 * hh, sg, tm_out, p);
       }
     }
   }
+  if (lane == 0) bulk_wait_group_all();  // output boxes complete before exit
 }
 
 template <typename T, int HD, bool PREFIX>
 __global__ void __launch_bounds__(GroupedSmem<HD>::kThreads, 1)
 grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                    const __grid_constant__ CUtensorMap tm_v, const GroupedParams p) {
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
+                    const GroupedParams p) {
   using L = GroupedSmem<HD>;
   constexpr int ST = L::kStages;
   constexpr int NT = L::kNT;
@@ -795,10 +831,10 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         int kv = 0;
         uint32_t pf_phase[2] = {0u, 0u}, q_phase[2] = {0u, 0u};
         bool ok = true;
+        Seg next = seg_of<PREFIX, NT>(item_of(0), p);
         for (int k = 0; ok; ++k) {
-          const int item = item_of(k);
-          if (item >= p.num_items) break;
-          const Seg s = seg_of<PREFIX, NT>(item, p);
+          if (item_of(k) >= p.num_items) break;
+          const Seg s = next;
           const int keys_a = tile_keys<PREFIX>(s, 0, p.positions);
           const int keys_b = NT == 2 ? tile_keys<PREFIX>(s, 1, p.positions) : 0;
           const int n_a = key_tiles(keys_a), n_b = key_tiles(keys_b), n = max(n_a, n_b);
@@ -827,6 +863,8 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             }
             __syncwarp();
           }
+          // the next item's place, while this one's first softmax runs
+          if (item_of(k + 1) < p.num_items) next = seg_of<PREFIX, NT>(item_of(k + 1), p);
           for (int j = 0; j < n; ++j) {
             const int st = (kv0 + j) % ST;
             const int st_n = (kv0 + j + 1) % ST;
@@ -882,9 +920,9 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   } else {
     setmaxnreg_inc<L::kRegsSoftmax>();
     if constexpr (kSepP)
-      softmax_pairs<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, s_full, s_free, p_full, o_done, abort_flag);
+      softmax_pairs<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, &tm_out, s_full, s_free, p_full, o_done, abort_flag);
     else
-      softmax_rows<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, s_full, p_full, o_done, abort_flag);
+      softmax_rows<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, &tm_out, s_full, p_full, o_done, abort_flag);
   }
   tc_fence_before();
   __syncthreads();
@@ -922,7 +960,7 @@ int launch_grouped(const GroupedTensors& x, const GroupedParams& p, cudaStream_t
   const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t hd = (uint64_t)p.hd, g = (uint64_t)p.group, hkv = (uint64_t)p.kv_heads;
-  CUtensorMap tm_q, tm_k, tm_v;
+  CUtensorMap tm_q, tm_k, tm_v, tm_out;
   {
     const uint64_t dims[4] = {hd, g, hkv, (uint64_t)x.q_rows};
     const uint64_t strides[3] = {(uint64_t)x.q_head_stride * 2, (uint64_t)x.q_head_stride * 2 * g,
@@ -936,11 +974,20 @@ int launch_grouped(const GroupedTensors& x, const GroupedParams& p, cudaStream_t
   const uint64_t vs[2] = {(uint64_t)x.v_head_stride * 2, (uint64_t)x.v_row_stride * 2};
   if (int rc = encode_tmap(&tm_k, dt, 3, x.k, dims, ks, box)) return rc;
   if (int rc = encode_tmap(&tm_v, dt, 3, x.v, dims, vs, box)) return rc;
+  if (p.box_store) {
+    // out [T][Hq][hd] as [T][kv heads][group][hd]: a softmax warp's rows, 64 columns
+    const uint64_t odims[4] = {hd, g, hkv, (uint64_t)x.q_rows};
+    const uint64_t ostr[3] = {hd * 2, hd * 2 * g, hd * 2 * g * hkv};
+    const uint32_t obox[4] = {64, (uint32_t)p.group, 1, (uint32_t)(L::kEpiRows / p.group)};
+    if (int rc = encode_tmap(&tm_out, dt, 4, p.out, odims, ostr, obox)) return rc;
+  } else {
+    tm_out = tm_q;  // not used
+  }
   auto kern = grouped_attn_kernel<T, HD, PREFIX>;
   static std::atomic<uint64_t> done{0};
   if (int rc = prepare_kernel(kern, L::kLaunchRegs, L::kTotal, done)) return rc;
   const int grid = p.num_items < sm_count() ? p.num_items : sm_count();
-  TTJ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(L::kThreads), L::kTotal, stream, tm_q, tm_k, tm_v, p));
+  TTJ_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(L::kThreads), L::kTotal, stream, tm_q, tm_k, tm_v, tm_out, p));
   return TTJ_OK;
 }
 
@@ -975,6 +1022,8 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
   // As in the dense kernel: when all heads' K and V exceed about 3/4 of the L2,
   // a head's items run consecutively and share its K/V there.
   p.head_major = a.tokens * a.num_kv_heads * a.head_dim * 4 > kHeadMajorKvBytes ? 1 : 0;
+  p.kv_shift = (p.kv_heads & (p.kv_heads - 1)) == 0 ? __builtin_ctz((unsigned)p.kv_heads) : -1;
+  p.box_store = (p.hd <= 64 ? 16 : 32) % p.group == 0;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   p.status = a.status;
   return dispatch<false>(a.dtype, x, p, stream);
