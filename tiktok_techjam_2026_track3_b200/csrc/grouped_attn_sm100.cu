@@ -60,7 +60,8 @@ struct GroupedParams {
   int num_heads, hd;
   int head_major;         // item order: 1 = a head's entries consecutive
   int kv_shift;           // log2 of kv_heads, or -1
-  int box_store;          // a softmax warp's rows are whole groups: its output rows form a TMA box
+  int box_store;          // head_dim 64: a softmax warp's rows are whole groups, its output a TMA box
+  int wide_store;         // head_dim above: output rows are 32-byte aligned
   int batch, prefix, split_keys, row_items;  // prefix: row_items = ceil(B / (tiles * positions))
   float scale_log2;
   int* status;
@@ -77,14 +78,16 @@ struct GroupedSmem {
   static constexpr uint32_t kRegsSoftmax = kSepP ? 104 : 184;
   static_assert(128 * kRegsCtl + (kThreads - 128) * kRegsSoftmax == kThreads * kLaunchRegs,
                 "register split must use the launch budget");
-  static constexpr int kEpiRows = kSepP ? 16 : 32;   // rows of a softmax warp's staging box
-  static constexpr int kStages = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  static constexpr int kEpiRows = kSepP ? 16 : 0;    // rows of a softmax warp's staging box
+  // K / V ring stages: what fits (K, which the tensor core needs first, takes the odd one)
+  static constexpr int kStagesK = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  static constexpr int kStagesV = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
   static constexpr int kTileBytes = HD * 2 * 128;
   static constexpr int kQBufs = HD == 64 ? 2 : 1;
   static constexpr int kQOff = 0;                    // [kQBufs][Q_A, Q_B]
   static constexpr int kKOff = kNT * kQBufs * kTileBytes;
-  static constexpr int kVOff = kKOff + kStages * kTileBytes;
-  static constexpr int kEpiOff = kVOff + kStages * kTileBytes;
+  static constexpr int kVOff = kKOff + kStagesK * kTileBytes;
+  static constexpr int kEpiOff = kVOff + kStagesV * kTileBytes;
   static constexpr int kBarOff = kEpiOff + (kThreads / 32 - 4) * kEpiRows * 128;
   static constexpr int kTotal = 1024 + kBarOff + 512;
   static_assert(kTotal <= 232448, "shared memory budget");
@@ -165,6 +168,11 @@ __device__ __forceinline__ int64_t row_index(int r, int pos, int t, const Seg& s
 template <bool PREFIX>
 __device__ __forceinline__ int row_limit(int pos, int t, const Seg& s, const GroupedParams& p) {
   return PREFIX ? s.nk - 1 : s.rel + t * p.positions + pos;
+}
+
+__device__ __forceinline__ void st_global_v8(void* to, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 // Store a staged box of ROWS rows x 64 columns (16-bit, 128-byte rows, swizzled): as
@@ -391,9 +399,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
 // Softmax, one warp per tile and TMEM lane quarter, thread = row, P over S
 // (head_dim 128 and 256).
 template <typename T, int HD, bool PREFIX>
-__device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* epi_base, uint32_t tmem,
-                                             const CUtensorMap* tm_out,
-                                             uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
+__device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint32_t tmem, uint64_t* s_full, uint64_t* p_full, uint64_t* o_done,
                                              volatile int* abort_flag) {
   using L = GroupedSmem<HD>;
   const int warp = threadIdx.x >> 5;
@@ -406,7 +412,6 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
   const uint32_t t_s = t_lane + t * 128;
   const uint32_t t_p = t_lane + L::kColP + t * L::kPStride;
   const uint32_t t_o = t_lane + L::kColO + t * HD;
-  const uint32_t box = smem_u32(epi_base) + (warp - 4) * (L::kEpiRows * 128);
   const int pos = row_pos(r, p);
   uint32_t sf_phase = 0, od_phase = 0;
   bool ok = true;
@@ -513,41 +518,48 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint8_t* ep
       for (int c = 0; c < HD / 32; ++c) {
         if (32 * c >= p.hd) break;  // uniform
         uint32_t o[32];
+        __syncwarp();
         tmem_ld32(t_o + c * 32, o);
         if (at >= 0) {
+          // (hd is a multiple of 8: every row of the workspace is 32-byte aligned)
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (32 * c + i < p.hd)
-              *reinterpret_cast<float4*>(part + 32 * c + i) =
-                  make_float4(__uint_as_float(o[i]) * inv_l, __uint_as_float(o[i + 1]) * inv_l,
-                              __uint_as_float(o[i + 2]) * inv_l, __uint_as_float(o[i + 3]) * inv_l);
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(__uint_as_float(o[i + e]) * inv_l);
+            if (32 * c + i < p.hd) st_global_v8(part + 32 * c + i, w);
+          }
         }
       }
     } else {
+      // A thread's row goes out as whole 32-byte sectors straight from its registers.
+      // (Staging 64 columns in shared memory for a TMA box took ~2300 cycles of an
+      // item's ~7000 with one key tile: two proxy fences and a wait for the box.)
+      T* out = static_cast<T*>(p.out) + at * p.hd;
 #pragma unroll 1
-      for (int hh = 0; hh < HD / 64; ++hh) {
-        if (64 * hh >= p.hd) break;  // only zero padding left (uniform)
-        box_free();
+      for (int c = 0; c < HD / 32; ++c) {
+        if (32 * c >= p.hd) break;  // uniform
+        uint32_t o[32];
+        __syncwarp();  // (rows of no position stored nothing in the last round)
+        tmem_ld32(t_o + c * 32, o);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + hh * 64 + c * 32, o);
+        for (int q = 0; q < 2; ++q) {
+          if (at < 0) break;
+          uint32_t w[8];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = Pack<T>::two(__uint_as_float(o[8 * q + 2 * i]) * inv_l, __uint_as_float(o[8 * q + 2 * i + 1]) * inv_l);
-            const int chunk = c * 4 + q;  // 16-byte chunk of the 128-byte row
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)),
-                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+          for (int i = 0; i < 8; ++i)
+            w[i] = Pack<T>::two(__uint_as_float(o[16 * q + 2 * i]) * inv_l, __uint_as_float(o[16 * q + 2 * i + 1]) * inv_l);
+          const int col = 32 * c + 16 * q;
+          if (p.wide_store && col + 16 <= p.hd) {
+            st_global_v8(out + col, w);
+          } else {
+            if (col < p.hd) *reinterpret_cast<uint4*>(out + col) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (col + 8 < p.hd) *reinterpret_cast<uint4*>(out + col + 8) = make_uint4(w[4], w[5], w[6], w[7]);
           }
         }
-        store_box<T, 32>(box, at, r0, t, 64 * hh, sg, tm_out, p);
       }
     }
   }
-  if (lane == 0) bulk_wait_group_all();  // output boxes complete before exit
 }
 
 template <typename T, int HD, bool PREFIX>
@@ -556,7 +568,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
                     const GroupedParams p) {
   using L = GroupedSmem<HD>;
-  constexpr int ST = L::kStages;
+  constexpr int SK = L::kStagesK, SV = L::kStagesV;
   constexpr int NT = L::kNT;
   constexpr bool kSepP = L::kSepP;
   constexpr int kChunks = HD / 64;
@@ -572,11 +584,11 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* q_full = bars;              // [kQBufs][2] per tile: Q_t loaded
   uint64_t* q_empty = q_full + 4;       // [kQBufs][2] per tile: last Q_t K^T of the item done
-  uint64_t* k_full = q_empty + 4;       // [ST]
-  uint64_t* k_empty = k_full + ST;      // [2][ST] per tile: its Q_t K^T done with the stage
-  uint64_t* v_full = k_empty + 2 * ST;  // [ST]
-  uint64_t* v_empty = v_full + ST;      // [2][ST] per tile: its P_t V done with the stage
-  uint64_t* s_full = v_empty + 2 * ST;  // [2] per tile: S_t written
+  uint64_t* k_full = q_empty + 4;       // [SK]
+  uint64_t* k_empty = k_full + SK;      // [2][SK] per tile: its Q_t K^T done with the stage
+  uint64_t* v_full = k_empty + 2 * SK;  // [SV]
+  uint64_t* v_empty = v_full + SV;      // [2][SV] per tile: its P_t V done with the stage
+  uint64_t* s_full = v_empty + 2 * SV;  // [2] per tile: S_t written
   uint64_t* s_free = s_full + 2;        // [2] per tile: S_t read by the softmax (separate P)
   uint64_t* p_full = s_free + 2;        // [2] per tile: P_t written
   uint64_t* o_done = p_full + 2;        // [2] per tile: one phase per completed P_t V (separate P) or item
@@ -589,13 +601,13 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   constexpr int kSoftmaxThreads = kSepP ? 256 : 128;  // per tile
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < SK; ++s) {
       mbar_init(&k_full[s], 1);
+      for (int t = 0; t < 2; ++t) mbar_init(&k_empty[t * SK + s], 1);
+    }
+    for (int s = 0; s < SV; ++s) {
       mbar_init(&v_full[s], 1);
-      for (int t = 0; t < 2; ++t) {
-        mbar_init(&k_empty[t * ST + s], 1);
-        mbar_init(&v_empty[t * ST + s], 1);
-      }
+      for (int t = 0; t < 2; ++t) mbar_init(&v_empty[t * SV + s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       for (int b = 0; b < 2; ++b) {
@@ -641,11 +653,11 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       // tile B's barriers).
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      auto reclaim = [&](uint64_t* empty, int kv) -> bool {
-        const int st = kv % ST;
-        const uint32_t phase = ((kv / ST) & 1) ^ 1;  // passes on the first round
+      auto reclaim = [&](uint64_t* empty, int stages, int kv) -> bool {
+        const int st = kv % stages;
+        const uint32_t phase = ((kv / stages) & 1) ^ 1;  // passes on the first round
         return (!kSepP || mbar_wait(&empty[st], phase, p.status, kDevTimeoutSmemEmpty, abort_flag)) &&
-               mbar_wait(&empty[ST + st], phase, p.status, kDevTimeoutSmemEmpty, abort_flag);
+               mbar_wait(&empty[stages + st], phase, p.status, kDevTimeoutSmemEmpty, abort_flag);
       };
       int kv = 0;  // running K/V tile counter across items
       bool ok = true;
@@ -655,15 +667,15 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const Seg s = seg_of<PREFIX, NT>(item, p);
         const int n_kv = item_tiles<PREFIX, NT>(s, p.positions);
         for (int j = 0; j < n_kv; ++j, ++kv) {
-          const int st = kv % ST;
-          if (!reclaim(k_empty, kv)) { ok = false; break; }
-          mbar_arrive_expect_tx(&k_full[st], L::kTileBytes);
+          const int sk = kv % SK, sv = kv % SV;
+          if (!reclaim(k_empty, SK, kv)) { ok = false; break; }
+          mbar_arrive_expect_tx(&k_full[sk], L::kTileBytes);
           for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(sK + st * L::kTileBytes + c * kChunkBytes, &tm_k, &k_full[st], 64 * c, s.kvh, s.k0 + j * kTile);
-          if (!reclaim(v_empty, kv)) { ok = false; break; }
-          mbar_arrive_expect_tx(&v_full[st], L::kTileBytes);
+            tma_load_3d(sK + sk * L::kTileBytes + c * kChunkBytes, &tm_k, &k_full[sk], 64 * c, s.kvh, s.k0 + j * kTile);
+          if (!reclaim(v_empty, SV, kv)) { ok = false; break; }
+          mbar_arrive_expect_tx(&v_full[sv], L::kTileBytes);
           for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(sV + st * L::kTileBytes + c * kChunkBytes, &tm_v, &v_full[st], 64 * c, s.kvh, s.k0 + j * kTile);
+            tma_load_3d(sV + sv * L::kTileBytes + c * kChunkBytes, &tm_v, &v_full[sv], 64 * c, s.kvh, s.k0 + j * kTile);
         }
       }
     } else if (warp == 2 && lane == 0) {
@@ -762,8 +774,8 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (!mbar_wait_warp(&s_free[t], sfree_ph, p.status, kDevTimeoutSoftmax, abort_flag)) return false;
             sfree_ph ^= 1u;
           }
-          const int st = qk_kv % ST;
-          if (!mbar_wait_warp(&k_full[st], (qk_kv / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
+          const int st = qk_kv % SK;
+          if (!mbar_wait_warp(&k_full[st], (qk_kv / SK) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
           ++qk_kv;
           const bool last = keys > 0 && keys <= kTile;  // the last S_t of the item: Q_t may be replaced
           if (keys > 0) {
@@ -771,12 +783,12 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (lane == 0) {
               qk(t, st, qb, keys);
               umma_commit(&s_full[t]);
-              umma_commit(&k_empty[t * ST + st]);
+              umma_commit(&k_empty[t * SK + st]);
               if (last) umma_commit(&q_empty[qb * 2 + t]);
             }
             qk_first = false;
           } else if (lane == 0) {
-            mbar_arrive(&k_empty[t * ST + st]);
+            mbar_arrive(&k_empty[t * SK + st]);
           }
           __syncwarp();
           if (last) ++qk_cnt;
@@ -798,8 +810,8 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               if (!mbar_wait_warp(&p_full[t], pf_ph, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
               pf_ph ^= 1u;
             }
-            const int st = kv % ST;
-            if (!mbar_wait_warp(&v_full[st], (kv / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            const int st = kv % SV;
+            if (!mbar_wait_warp(&v_full[st], (kv / SV) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
             if (active) {
               // both tiles' issuers may write these zeros; a product that already
               // reads them reads zeros either way
@@ -808,10 +820,10 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               if (lane == 0) {
                 pv(t, st, j > 0, keys - j * kTile);
                 umma_commit(&o_done[t]);
-                umma_commit(&v_empty[t * ST + st]);
+                umma_commit(&v_empty[t * SV + st]);
               }
             } else if (lane == 0) {
-              mbar_arrive(&v_empty[t * ST + st]);
+              mbar_arrive(&v_empty[t * SV + st]);
             }
             __syncwarp();
           }
@@ -847,8 +859,8 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           }
           const int kv0 = kv;
           {
-            const int st = kv0 % ST;
-            if (!mbar_wait_warp(&k_full[st], (kv0 / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) break;
+            const int st = kv0 % SK;
+            if (!mbar_wait_warp(&k_full[st], (kv0 / SK) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) break;
             tc_fence_after();
             if (lane == 0) {
               qk(0, st, 0, keys_a);
@@ -859,19 +871,19 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 umma_commit(&s_full[1]);
                 if (n_b == 1) umma_commit(&q_empty[1]);
               }
-              umma_commit(&k_empty[ST + st]);
+              umma_commit(&k_empty[SK + st]);
             }
             __syncwarp();
           }
           // the next item's place, while this one's first softmax runs
           if (item_of(k + 1) < p.num_items) next = seg_of<PREFIX, NT>(item_of(k + 1), p);
           for (int j = 0; j < n; ++j) {
-            const int st = (kv0 + j) % ST;
-            const int st_n = (kv0 + j + 1) % ST;
+            const int st = (kv0 + j) % SV;
+            const int st_n = (kv0 + j + 1) % SK;
             const int left = nk - j * kTile;  // keys of the item from this tile on
-            if (j + 1 < n && !mbar_wait_warp(&k_full[st_n], ((kv0 + j + 1) / ST) & 1, p.status, kDevTimeoutTmaFull,
+            if (j + 1 < n && !mbar_wait_warp(&k_full[st_n], ((kv0 + j + 1) / SK) & 1, p.status, kDevTimeoutTmaFull,
                                              abort_flag)) { ok = false; break; }
-            if (!mbar_wait_warp(&v_full[st], ((kv0 + j) / ST) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            if (!mbar_wait_warp(&v_full[st], ((kv0 + j) / SV) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
             if (left < kTile) zero_v_tail(st, left);
             if (j < n_a) {
               if (!mbar_wait_warp(&p_full[0], pf_phase[0], p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
@@ -896,7 +908,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             }
             if (lane == 0) {
               if (j < n_b) pv(1, st, j > 0, keys_b - j * kTile);
-              umma_commit(&v_empty[ST + st]);
+              umma_commit(&v_empty[SV + st]);
               if (j + 1 < n_b) {
                 qk(1, st_n, 0, keys_b - (j + 1) * kTile);
                 umma_commit(&s_full[1]);
@@ -904,7 +916,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               } else if (j < n_b) {
                 umma_commit(&o_done[1]);
               }
-              if (j + 1 < n) umma_commit(&k_empty[ST + st_n]);
+              if (j + 1 < n) umma_commit(&k_empty[SK + st_n]);
             }
             __syncwarp();
           }
@@ -922,7 +934,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     if constexpr (kSepP)
       softmax_pairs<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, &tm_out, s_full, s_free, p_full, o_done, abort_flag);
     else
-      softmax_rows<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, &tm_out, s_full, p_full, o_done, abort_flag);
+      softmax_rows<T, HD, PREFIX>(p, tmem, s_full, p_full, o_done, abort_flag);
   }
   tc_fence_before();
   __syncthreads();
@@ -978,7 +990,7 @@ int launch_grouped(const GroupedTensors& x, const GroupedParams& p, cudaStream_t
     // out [T][Hq][hd] as [T][kv heads][group][hd]: a softmax warp's rows, 64 columns
     const uint64_t odims[4] = {hd, g, hkv, (uint64_t)x.q_rows};
     const uint64_t ostr[3] = {hd * 2, hd * 2 * g, hd * 2 * g * hkv};
-    const uint32_t obox[4] = {64, (uint32_t)p.group, 1, (uint32_t)(L::kEpiRows / p.group)};
+    const uint32_t obox[4] = {64, (uint32_t)p.group, 1, (uint32_t)(16 / p.group)};
     if (int rc = encode_tmap(&tm_out, dt, 4, p.out, odims, ostr, obox)) return rc;
   } else {
     tm_out = tm_q;  // not used
@@ -1023,7 +1035,8 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
   // a head's items run consecutively and share its K/V there.
   p.head_major = a.tokens * a.num_kv_heads * a.head_dim * 4 > kHeadMajorKvBytes ? 1 : 0;
   p.kv_shift = (p.kv_heads & (p.kv_heads - 1)) == 0 ? __builtin_ctz((unsigned)p.kv_heads) : -1;
-  p.box_store = (p.hd <= 64 ? 16 : 32) % p.group == 0;
+  p.box_store = p.hd <= 64 && 16 % p.group == 0;
+  p.wide_store = p.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   p.status = a.status;
   return dispatch<false>(a.dtype, x, p, stream);
