@@ -397,6 +397,8 @@ typedef struct ttj_shared_prefix_attn_args {
   const float* key_weights;        /* [B, num_kv_heads, C] or NULL */
   float* key_weights_out;          /* same shape, aliases no input; required with key_weights */
   void* out;                       /* [B, num_heads, head_dim] contiguous */
+  float* lse;                      /* [B, num_heads] log of each row's sum of exponentials (-inf
+                                      without any key), or NULL */
   void* workspace;
   size_t workspace_bytes;
   int* status;

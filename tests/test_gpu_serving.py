@@ -421,3 +421,19 @@ def test_serving_ops_on_a_side_stream_and_in_a_graph():
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_decode_lse_joins_two_key_sets():
+    """return_lse: the results over the prefix and over the caches join to the result over both."""
+    q, pk, pv, kc, vc = decode_case(5, 150, 90, 8, 2, 128, torch.float16, 21)
+    lens = torch.tensor([90, 0, 1, 44, 64], dtype=torch.int32).cuda()
+    both, lse = ops.shared_prefix_attn(q, pk, pv, kc, vc, lens, return_lse=True)
+    a, la = ops.shared_prefix_attn(q, pk, pv, kc[:, :0], vc[:, :0], lens, return_lse=True)
+    b, neww, lb = ops.shared_prefix_attn(q, pk[:0], pv[:0], kc, vc, lens, key_weights=torch.zeros(5, 2, 90).cuda(),
+                                         return_lse=True)
+    assert bool((lb[1] == -math.inf).all()) and neww.shape == (5, 2, 90)
+    assert float((torch.logaddexp(la, lb) - lse).abs().max()) <= 2e-5 * (1 + float(lse.abs().max()))
+    wa, wb = torch.exp(la - lse)[..., None], torch.exp(lb - lse)[..., None]
+    # three roundings to fp16 of values below max |v|, each probability rounded once more
+    tol = 4 * 2.0 ** -11 * float(torch.cat([pv.flatten(), vc.flatten()]).abs().max())
+    assert float((wa * a.float() + wb * b.float() - both.float()).abs().max()) <= tol

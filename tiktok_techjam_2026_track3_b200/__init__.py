@@ -10,5 +10,6 @@ kernel.  No CPU fallback: without the built library every op raises.
 from . import ops  # noqa: F401
 from .config import PRESETS, LayerConfig, attention_flops  # noqa: F401
 from .layer import B200AttentionLayer, B200SelfAttention  # noqa: F401
+from .serving import CachedAttention, SequenceCache, SharedPrefix  # noqa: F401
 
 __version__ = "0.1.0"

@@ -96,7 +96,7 @@ class SharedPrefixAttnArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("prefix_k", vp), ("prefix_v", vp), ("k_cache", vp), ("v_cache", vp),
         ("lengths", vp), ("key_weights", vp), ("key_weights_out", vp), ("out", vp),
-        ("workspace", vp), ("workspace_bytes", C.c_size_t), ("status", vp),
+        ("lse", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t), ("status", vp),
         ("batch", i64), ("prefix_len", i64), ("capacity", i64), ("num_heads", i64),
         ("num_kv_heads", i64), ("head_dim", i64),
         ("q_seq_stride", i64), ("q_head_stride", i64),

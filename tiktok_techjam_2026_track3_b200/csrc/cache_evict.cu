@@ -14,7 +14,10 @@
 //    above / equal counting the earlier rows with a larger / an equal key: equal rows
 //    are kept lowest index first by construction.
 //    (Digit histograms in shared memory took 33 us for 512 caches of 4096 rows and
-//    81 us for 32 of 65537 where this takes CHOOSE_BATCH and CHOOSE_LONG.)
+//    81 us for 32 of 65537 where this takes 25 and 40.  A counting pass costs ~1000
+//    cycles of instruction issue per resident set of blocks, a cluster barrier as
+//    much again; blocks of 256 threads with a one-warp or an all-pairs end of the
+//    search, and a fourth resident block, measured 0 to 5% slower.)
 // 2. Copying (bound by the kept rows' bytes): a warp takes 32 output rows in the
 //    order of the output's memory and copies K and V rows in 16-byte pieces, eight
 //    rows in flight.
@@ -69,11 +72,11 @@ struct Cut {
   int bits, at, above;
   __device__ __forceinline__ uint32_t candidate(int q) const { return cut | ((uint32_t)q << (bits - 2)); }
   __device__ __forceinline__ void take(int n1, int n2, int n3, int need) {
-    const int n[3] = {n1, n2, n3};
-    int q = n3 >= need ? 3 : (n2 >= need ? 2 : (n1 >= need ? 1 : 0));
-    if (q < 3) above = n[q];
-    if (q > 0) at = n[q - 1];
-    cut = candidate(q);
+    const uint32_t c1 = candidate(1), c2 = candidate(2), c3 = candidate(3);
+    if (n3 >= need) at = n3, cut = c3;
+    else if (n2 >= need) at = n2, cut = c2, above = n3;
+    else if (n1 >= need) at = n1, cut = c1, above = n2;
+    else above = n1;
     bits -= 2;
   }
 };
@@ -192,15 +195,16 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
       // the keys in [cut, cut + 2^bits), collected by the first block
       uint32_t* list = cluster.map_shared_rank(s_list, 0);
       int* listed = cluster.map_shared_rank(&s_listed, 0);
+      auto in_list = [&](uint32_t k) { return k != 0u && (k ^ x.cut) >> x.bits == 0u; };  // bits <= 30 here
+      int mine = 0, at = 0;
+      each([&](int, uint32_t k) { mine += __popc(__ballot_sync(0xffffffffu, in_list(k))); });
+      if (lane == 0 && mine > 0) at = atomicAdd(listed, mine);
+      at = __shfl_sync(0xffffffffu, at, 0);
       each([&](int, uint32_t k) {
-        const bool in = k != 0u && (k ^ x.cut) >> x.bits == 0u;  // bits <= 30 here
+        const bool in = in_list(k);
         const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (who != 0u) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(listed, __popc(who));
-          at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-          if (in) list[at] = k;
-        }
+        if (in) list[at + __popc(who & ((1u << lane) - 1u))] = k;
+        at += __popc(who);
       });
       sync_all();
       const int count = x.at - x.above;

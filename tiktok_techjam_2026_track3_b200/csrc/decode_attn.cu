@@ -474,6 +474,7 @@ struct JoinParams {
   const float *scores, *key_weights;
   float* key_weights_out;
   void* out;
+  float* lse;                          // [B][Hq] or null
   const int32_t* lengths;
   int64_t score_pitch, rows, out_blocks;
   int spans, span;                     // spans of `span` cached keys
@@ -604,6 +605,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
+      if (p.lse != nullptr && col0 == 0 && lane == 0) p.lse[row] = (top + log2f(sum)) * 0.69314718055994531f;
       if (col < p.hd)
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * p.hd + col) =
             make_uint2(Pack<T>::two(v.x * inv, v.y * inv), Pack<T>::two(v.z * inv, v.w * inv));
@@ -810,6 +812,7 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   j.key_weights = a.key_weights;
   j.key_weights_out = a.key_weights_out;
   j.out = a.out;
+  j.lse = a.lse;
   j.lengths = a.lengths;
   j.score_pitch = w.pitch;
   j.rows = a.batch * a.num_heads;

@@ -523,15 +523,18 @@ def _dense(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtype: torch.dtyp
 def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
                        k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                        key_weights: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                       out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+                       return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                       workspace: Optional[torch.Tensor] = None):
     """One decode step: each sequence's new token q [B,Hq,hd] attends the prefix rows
     prefix_k / prefix_v [P,Hkv,hd] that the whole batch shares, then the first
     ``lengths[b]`` rows of its own cache k_cache / v_cache [B,C,Hkv,hd] (P and C may
-    be zero; a sequence without any key gets zeros).  Returns [B,Hq,hd].
+    be zero; a sequence without any key gets zeros).  Returns [B,Hq,hd], followed by
+    whichever of these is asked for:
 
-    With ``key_weights`` (fp32 [B,Hkv,C]) it returns (out, new_key_weights): each
-    cached key's weight plus this step's probabilities of that key summed over
-    the group's heads, for ``cache_evict``; the input is not written."""
+    ``key_weights`` (fp32 [B,Hkv,C]) gives new_key_weights, each cached key's weight
+    plus this step's probabilities of that key summed over the group's heads, for
+    ``cache_evict`` (the input is not written); ``return_lse`` gives the log of each
+    row's sum of exponentials, fp32 [B,Hq], -inf for a row without any key."""
     dt = _dtype_code(q)
     if q.dim() != 3 or prefix_k.dim() != 3 or k_cache.dim() != 4:
         raise RuntimeError("q must be [B,Hq,hd], prefix_k and prefix_v [P,Hkv,hd], k_cache and v_cache [B,C,Hkv,hd]")
@@ -561,14 +564,17 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
         out = q.new_empty((B, Hq, hd))
     elif out.shape != (B, Hq, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     need = _lib.load().ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, key_weights is not None)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     _launch(_lib.shared_prefix_attn_fwd, dev, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
-            _ptr(new_weights) or 0, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+            _ptr(new_weights) or 0, out.data_ptr(), _ptr(lse) or 0, workspace.data_ptr(), workspace.numel(),
             status_word(dev).data_ptr(), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
             hd ** -0.5 if scale is None else float(scale), dt)
-    return out if new_weights is None else (out, new_weights)
+    if new_weights is None and lse is None:
+        return out
+    return (out,) + tuple(t for t in (new_weights, lse) if t is not None)
 
 
 class EvictedCache(NamedTuple):
