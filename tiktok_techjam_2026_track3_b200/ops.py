@@ -8,6 +8,7 @@ any error code.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Dict, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -520,6 +521,13 @@ def _dense(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtype: torch.dtyp
     return t if t.is_contiguous() else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(B: int, P: int, Cap: int, Hq: int, Hkv: int, hd: int, weights: bool, index: int) -> int:
+    """Bytes of workspace of a decode step of these sizes on device `index`."""
+    with torch.cuda.device(index):
+        return _lib.load().ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, weights)
+
+
 def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
                        k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                        key_weights: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -565,12 +573,12 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     elif out.shape != (B, Hq, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    need = _lib.load().ttj_shared_prefix_attn_workspace_size(B, P, Cap, Hq, Hkv, hd, key_weights is not None)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    need = _decode_workspace(B, P, Cap, Hq, Hkv, hd, key_weights is not None, dev.index)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = lengths.new_empty((need // 4,))   # (a multiple of 256 bytes)
     _launch(_lib.shared_prefix_attn_fwd, dev, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
-            _ptr(new_weights) or 0, out.data_ptr(), _ptr(lse) or 0, workspace.data_ptr(), workspace.numel(),
-            status_word(dev).data_ptr(), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
+            _ptr(new_weights) or 0, out.data_ptr(), _ptr(lse) or 0, workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), status_word(dev).data_ptr(), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
             hd ** -0.5 if scale is None else float(scale), dt)
     if new_weights is None and lse is None:
         return out
@@ -613,16 +621,20 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
     if out is None:
         k_out = k_cache.new_empty((B, budget, Hkv, hd))
         v_out = k_cache.new_empty((B, budget, Hkv, hd))
+        kop, vop = k_out.data_ptr(), v_out.data_ptr()
+        koh = voh = hd
+        kor = vor = Hkv * hd
+        kos = vos = budget * kor
     else:
         k_out, v_out = out
         _same(k_cache, k_out=k_out, v_out=v_out)
         for t, n in ((k_out, "k_out"), (v_out, "v_out")):
             if t.dim() != 4 or t.shape[0] != B or t.shape[1] < budget or t.shape[2:] != (Hkv, hd):
                 raise RuntimeError(f"{n} must be [{B}, >={budget}, {Hkv}, {hd}], got {list(t.shape)}")
-    ko, kop, kos, kor, koh = _strided(k_out, "k_out")
-    vo, vop, vos, vor, voh = _strided(v_out, "v_out")
-    if ko is not k_out or vo is not v_out:
-        raise RuntimeError("out must have contiguous rows and 16-byte aligned strides")
+        ko, kop, kos, kor, koh = _strided(k_out, "k_out")
+        vo, vop, vos, vor, voh = _strided(v_out, "v_out")
+        if ko is not k_out or vo is not v_out:
+            raise RuntimeError("out must have contiguous rows and 16-byte aligned strides")
     weights = key_weights.new_empty((B, Hkv, budget))
     new_lengths = lengths.new_empty((B,))
     positions = lengths.new_empty((B, Hkv, budget))
