@@ -35,6 +35,10 @@ constexpr int kWarps = 4;
 constexpr int kJoinThreads = 256;
 constexpr int kWeightStep = 1024;  // cached keys per join block and step
 constexpr int kMinSteps = 2;       // of a stretch
+// Beside the prefix kernel: up to kShareWaves times as many blocks as stay resident (2
+// times 264 us for 128 caches of up to 4096 keys, 4: 261, 8: 251, 16: 260), with
+// stretches of at least kShareSteps.
+constexpr int kShareWaves = 8, kShareSteps = 8;
 
 // NR: row tiles of 8 (group heads) that a warp carries, 1 or 2.
 template <int HD, int NR>
@@ -52,7 +56,8 @@ int line_blocks_per_sm(int64_t hd) { return hd > 128 ? 1 : (hd > 64 ? 2 : 3); }
 // How the step is cut (host).
 struct Cuts {
   bool prefix_tiles;        // prefix on the 128-row tensor-core kernel, in
-  int tile_parts, tile_keys;  // tile_parts ranges of tile_keys keys
+  int tile_parts, tile_keys;  // tile_parts ranges of tile_keys keys, on
+  int tile_blocks;          // at most this many blocks (one per SM)
   int blocks;               // of the line's grid; workers = blocks * kWarps / heads
   int tile_rows;            // rows of a warp's tile, 8 or 16
   int prefix_row_tiles;     // row tiles of the batch x group rows when the line has the prefix, else 0
@@ -149,8 +154,9 @@ line_kernel(const LineParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t s_before[kWarps * 32 + 1];  // steps before each thread's sequences, and of all
   // Behind the prefix kernel of the same step nothing of that kernel is read, and it
-  // has let this one start only once everything before it was complete: the wait
-  // moves to the end, where it keeps the join behind both.
+  // has let this one start only once everything before it was complete: only block 0
+  // waits, at its end, which keeps this grid's end, and so the join, behind both (a
+  // block that waits holds its place on the SM).
   if (!p.after_prefix) grid_dependency_wait();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -203,7 +209,7 @@ line_kernel(const LineParams p) {
   const int64_t from = worker * stretch;
   const int steps = (int)min(stretch, total - from);
   if (steps <= 0) {  // uniform over the warp; no block barrier follows
-    if (p.after_prefix) grid_dependency_wait();
+    if (p.after_prefix && blockIdx.x == 0) grid_dependency_wait();
     return;
   }
 
@@ -464,7 +470,7 @@ line_kernel(const LineParams p) {
     }
     if (i + 1 < steps) advance(at);
   }
-  if (p.after_prefix) grid_dependency_wait();
+  if (p.after_prefix && blockIdx.x == 0) grid_dependency_wait();
 }
 
 struct JoinParams {
@@ -675,7 +681,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads, int64_t kv_heads, int64_t hd) {
   Cuts c{};
   const int64_t group = num_heads / kv_heads, rows = batch * group;
-  c.prefix_tiles = prefix > 0 && rows > 32;
+  // A short prefix under few rows goes in the line, which saves a launch (512 keys, 8
+  // rows: 12.4 us a step against 14.4; 128 keys 10.9 against 14.4); beyond, the line
+  // leaves many partial results of little work each (16 rows, 4096 keys: 28.7 us
+  // against 16.4 on the tiles; 32 rows, 32768 keys: 63.8 against 25.1).
+  c.prefix_tiles = prefix > 0 && (prefix > 512 || rows > 16);
   const int64_t tile = (c.prefix_tiles || prefix == 0 ? group : rows) <= 8 ? 8 : 16;
   c.tile_rows = (int)tile;
   c.prefix_row_tiles = prefix > 0 && !c.prefix_tiles ? (int)ceil_div(rows, tile) : 0;
@@ -690,14 +700,34 @@ Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads,
   c.blocks = (int)std::min<int64_t>(line_blocks_per_sm(hd) * (int64_t)sm_count(),
                                     ceil_div(steps * c.heads, kMinSteps * kWarps));
   if (!c.prefix_tiles) return c;
-  // Persistent blocks, one per SM: the number of ranges with the least time, in key
-  // tiles of 128: waves x (tiles of a range + about 2 for its start and end).
+  // The two kernels share the GPU: the prefix's persistent blocks (one per SM) leave
+  // the caches' blocks the SMs that their work is worth, by a key tile's ~1.9 us and
+  // ~80 GB/s that an SM streams, caches taken as 0.6 full; as blocks of either end,
+  // the line's take their place.  (Each kernel on the whole GPU in turn: 64 sequences
+  // behind 32768 keys 74 us a step, now 66; 128 over up to 4096 cached keys
+  // 267 us, now 251; with caches a third full 88 us, now 91.)  Steps of less than
+  // ~20 us in all gain nothing (33 sequences of up to 2100 keys: 47 us, shared 53).
   const int64_t units = kv_heads * ceil_div(batch, plan_positions(group, hd)), tiles = ceil_div(prefix, 128);
+  const double prefix_us = 1.9 * (double)(units * tiles);
+  const double line_us = 0.6 * 4.0 * (double)(batch * kv_heads * c.cache_row_tiles) * (double)(capacity * hd) / 80e3;
+  const int sms = sm_count();
+  const int64_t want = (int64_t)(sms * prefix_us / (prefix_us + line_us) + 0.5);
+  c.tile_blocks = prefix_us + line_us < 20. * sms
+                      ? sms
+                      : (int)std::max<int64_t>(std::min<int64_t>(want, sms), std::min(24, sms));
+  // The number of ranges with the least time, in key tiles of 128: waves x (tiles of a
+  // range + about 2 for its start and end).
+  if (c.tile_blocks < sms) {
+    // the line's blocks start as SMs become free: shorter stretches even out their ends
+    const int64_t whole = steps * c.heads;
+    c.blocks = (int)std::max<int64_t>(c.blocks, std::min<int64_t>(kShareWaves * line_blocks_per_sm(hd) * (int64_t)sms,
+                                                                  whole / (kShareSteps * kWarps)));
+  }
   int64_t best = 1, best_time = INT64_MAX;
   for (int64_t n = 1; n <= std::min<int64_t>(tiles, 64); ++n) {
     const int64_t per = ceil_div(tiles, n);
     if (ceil_div(tiles, per) != n) continue;
-    const int64_t time = ceil_div(units * n, sm_count()) * (per + 2) * 16 + n;
+    const int64_t time = ceil_div(units * n, c.tile_blocks) * (per + 2) * 16 + n;
     if (time < best_time) best_time = time, best = n;
   }
   c.tile_keys = (int)(ceil_div(tiles, best) * 128);
@@ -758,7 +788,7 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   float* tile_lse = reinterpret_cast<float*>(ws + w.tile_lse);
   const int64_t group = a.num_heads / a.num_kv_heads;
   if (c.prefix_tiles)
-    if (int rc = launch_prefix_parts(a, tile_o, tile_lse, c.tile_parts, c.tile_keys, stream)) return rc;
+    if (int rc = launch_prefix_parts(a, tile_o, tile_lse, c.tile_parts, c.tile_keys, c.tile_blocks, stream)) return rc;
   LineParams p{};
   p.q = a.q;
   p.pk = a.prefix_k;

@@ -141,9 +141,10 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream);
 size_t shared_prefix_attn_workspace(int64_t batch, int64_t prefix_len, int64_t capacity, int64_t num_heads,
                                     int64_t num_kv_heads, int64_t head_dim, bool with_key_weights);
 // The prefix in `parts` ranges of part_keys keys (a multiple of 128): normalised
-// fp32 outputs part_o [parts][B][Hq][hd] and log2 of the sums part_lse [parts][B][Hq].
+// fp32 outputs part_o [parts][B][Hq][hd] and log2 of the sums part_lse [parts][B][Hq],
+// on at most max_blocks persistent blocks.
 int launch_prefix_parts(const ttj_shared_prefix_attn_args& a, float* part_o, float* part_lse, int parts,
-                        int part_keys, cudaStream_t stream);
+                        int part_keys, int max_blocks, cudaStream_t stream);
 int launch_shared_prefix_attn(const ttj_shared_prefix_attn_args& a, cudaStream_t stream);
 int launch_cache_evict(const ttj_cache_evict_args& a, cudaStream_t stream);
 
