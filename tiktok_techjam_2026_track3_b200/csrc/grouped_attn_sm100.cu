@@ -79,9 +79,12 @@ struct GroupedSmem {
   static_assert(128 * kRegsCtl + (kThreads - 128) * kRegsSoftmax == kThreads * kLaunchRegs,
                 "register split must use the launch budget");
   static constexpr int kEpiRows = kSepP ? 16 : 0;    // rows of a softmax warp's staging box
-  // K / V ring stages: what fits (K, which the tensor core needs first, takes the odd one)
-  static constexpr int kStagesK = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  // K / V ring stages: what fits.  With one K stage more than V stages, K_m may be
+  // loaded once V_{m-1} could be, as both wait for step m - 3 or earlier: K needs no
+  // release barrier of its own (a commit less for the MMA warp, ~100 cycles a step).
+  static constexpr int kStagesK = HD == 64 ? 4 : (HD == 128 ? 3 : 1);
   static constexpr int kStagesV = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  static constexpr bool kReleaseK = kStagesK != kStagesV + 1;
   static constexpr int kTileBytes = HD * 2 * 128;
   static constexpr int kQBufs = HD == 64 ? 2 : 1;
   static constexpr int kQOff = 0;                    // [kQBufs][Q_A, Q_B]
@@ -668,7 +671,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int n_kv = item_tiles<PREFIX, NT>(s, p.positions);
         for (int j = 0; j < n_kv; ++j, ++kv) {
           const int sk = kv % SK, sv = kv % SV;
-          if (!reclaim(k_empty, SK, kv)) { ok = false; break; }
+          if (L::kReleaseK && !reclaim(k_empty, SK, kv)) { ok = false; break; }
           mbar_arrive_expect_tx(&k_full[sk], L::kTileBytes);
           for (int c = 0; c < kChunks; ++c)
             tma_load_3d(sK + sk * L::kTileBytes + c * kChunkBytes, &tm_k, &k_full[sk], 64 * c, s.kvh, s.k0 + j * kTile);
@@ -851,16 +854,20 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const int keys_b = NT == 2 ? tile_keys<PREFIX>(s, 1, p.positions) : 0;
           const int n_a = key_tiles(keys_a), n_b = key_tiles(keys_b), n = max(n_a, n_b);
           const int nk = s.nk;
-          if (!mbar_wait_warp(&q_full[0], q_phase[0], p.status, kDevTimeoutTmaFull, abort_flag)) break;
-          q_phase[0] ^= 1u;
-          if (n_b > 0) {
-            if (!mbar_wait_warp(&q_full[1], q_phase[1], p.status, kDevTimeoutTmaFull, abort_flag)) break;
-            q_phase[1] ^= 1u;
-          }
           const int kv0 = kv;
           {
             const int st = kv0 % SK;
-            if (!mbar_wait_warp(&k_full[st], (kv0 / SK) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) break;
+            const uint32_t k_phase = (kv0 / SK) & 1;
+            const bool ready = mbar_try_wait(smem_u32(&q_full[0]), q_phase[0]) &
+                               (n_b == 0 || mbar_try_wait(smem_u32(&q_full[1]), q_phase[1])) &
+                               mbar_try_wait(smem_u32(&k_full[st]), k_phase);
+            if (!__all_sync(0xffffffffu, ready)) {
+              if (!mbar_wait_warp(&q_full[0], q_phase[0], p.status, kDevTimeoutTmaFull, abort_flag)) break;
+              if (n_b > 0 && !mbar_wait_warp(&q_full[1], q_phase[1], p.status, kDevTimeoutTmaFull, abort_flag)) break;
+              if (!mbar_wait_warp(&k_full[st], k_phase, p.status, kDevTimeoutTmaFull, abort_flag)) break;
+            }
+            q_phase[0] ^= 1u;
+            if (n_b > 0) q_phase[1] ^= 1u;
             tc_fence_after();
             if (lane == 0) {
               qk(0, st, 0, keys_a);
@@ -871,7 +878,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 umma_commit(&s_full[1]);
                 if (n_b == 1) umma_commit(&q_empty[1]);
               }
-              umma_commit(&k_empty[SK + st]);
+              if constexpr (L::kReleaseK) umma_commit(&k_empty[SK + st]);
             }
             __syncwarp();
           }
@@ -925,7 +932,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               } else if (j < n_b) {
                 umma_commit(&o_done[1]);
               }
-              if (j + 1 < n) umma_commit(&k_empty[SK + st_n]);
+              if (L::kReleaseK && j + 1 < n) umma_commit(&k_empty[SK + st_n]);
             }
             __syncwarp();
           }
