@@ -770,15 +770,20 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           if (!qk_live) return true;
           const int keys = qk_keys - qk_j * kTile;  // this tile's keys from here on
           const int qb = qk_cnt % L::kQBufs;
-          if (keys > 0 && qk_j == 0 &&
-              !mbar_wait_warp(&q_full[qb * 2 + t], (qk_cnt / L::kQBufs) & 1, p.status, kDevTimeoutTmaFull, abort_flag))
-            return false;
-          if (keys > 0 && !qk_first) {
-            if (!mbar_wait_warp(&s_free[t], sfree_ph, p.status, kDevTimeoutSoftmax, abort_flag)) return false;
-            sfree_ph ^= 1u;
-          }
+          // the barriers of this product, polled together (a completed wait costs this
+          // warp ~125 cycles)
           const int st = qk_kv % SK;
-          if (!mbar_wait_warp(&k_full[st], (qk_kv / SK) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
+          const uint32_t q_phase = (qk_cnt / L::kQBufs) & 1, k_phase = (qk_kv / SK) & 1;
+          const bool need_q = keys > 0 && qk_j == 0, need_s = keys > 0 && !qk_first;
+          const bool ready = (!need_q || mbar_try_wait(smem_u32(&q_full[qb * 2 + t]), q_phase)) &
+                             (!need_s || mbar_try_wait(smem_u32(&s_free[t]), sfree_ph)) &
+                             mbar_try_wait(smem_u32(&k_full[st]), k_phase);
+          if (!__all_sync(0xffffffffu, ready)) {
+            if (need_q && !mbar_wait_warp(&q_full[qb * 2 + t], q_phase, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
+            if (need_s && !mbar_wait_warp(&s_free[t], sfree_ph, p.status, kDevTimeoutSoftmax, abort_flag)) return false;
+            if (!mbar_wait_warp(&k_full[st], k_phase, p.status, kDevTimeoutTmaFull, abort_flag)) return false;
+          }
+          if (need_s) sfree_ph ^= 1u;
           ++qk_kv;
           const bool last = keys > 0 && keys <= kTile;  // the last S_t of the item: Q_t may be replaced
           if (keys > 0) {
@@ -809,12 +814,15 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           for (int j = 0; j < n; ++j, ++kv) {
             if (!issue_qk()) { ok = false; break; }
             const bool active = j * kTile < keys;
-            if (active) {
-              if (!mbar_wait_warp(&p_full[t], pf_ph, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
-              pf_ph ^= 1u;
-            }
             const int st = kv % SV;
-            if (!mbar_wait_warp(&v_full[st], (kv / SV) & 1, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            const uint32_t v_phase = (kv / SV) & 1;
+            const bool ready = (!active || mbar_try_wait(smem_u32(&p_full[t]), pf_ph)) &
+                               mbar_try_wait(smem_u32(&v_full[st]), v_phase);
+            if (!__all_sync(0xffffffffu, ready)) {
+              if (active && !mbar_wait_warp(&p_full[t], pf_ph, p.status, kDevTimeoutSoftmax, abort_flag)) { ok = false; break; }
+              if (!mbar_wait_warp(&v_full[st], v_phase, p.status, kDevTimeoutTmaFull, abort_flag)) { ok = false; break; }
+            }
+            if (active) pf_ph ^= 1u;
             if (active) {
               // both tiles' issuers may write these zeros; a product that already
               // reads them reads zeros either way
