@@ -83,7 +83,7 @@ struct GroupedSmem {
   // loaded once V_{m-1} could be, as both wait for step m - 3 or earlier: K needs no
   // release barrier of its own (a commit less for the MMA warp, ~100 cycles a step).
   static constexpr int kStagesK = HD == 64 ? 4 : (HD == 128 ? 3 : 1);
-  static constexpr int kStagesV = HD == 64 ? 4 : (HD == 128 ? 2 : 1);
+  static constexpr int kStagesV = HD == 64 ? 3 : (HD == 128 ? 2 : 1);
   static constexpr bool kReleaseK = kStagesK != kStagesV + 1;
   static constexpr int kTileBytes = HD * 2 * 128;
   static constexpr int kQBufs = HD == 64 ? 2 : 1;
@@ -791,11 +791,11 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (lane == 0) {
               qk(t, st, qb, keys);
               umma_commit(&s_full[t]);
-              umma_commit(&k_empty[t * SK + st]);
+              if constexpr (L::kReleaseK) umma_commit(&k_empty[t * SK + st]);
               if (last) umma_commit(&q_empty[qb * 2 + t]);
             }
             qk_first = false;
-          } else if (lane == 0) {
+          } else if (L::kReleaseK && lane == 0) {
             mbar_arrive(&k_empty[t * SK + st]);
           }
           __syncwarp();
