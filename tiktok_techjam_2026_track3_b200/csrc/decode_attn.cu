@@ -12,8 +12,10 @@
 // partial result.  A group has few rows (group heads), so the products run on warp
 // tiles of 8 or 16 rows.  Cache rows past the length are never read: their copies are
 // zero-filled.  (One block per cache range of at most 1024 keys, joined through
-// shared memory, took 36 us where the line takes LINE_UNGROUPED for 33 sequences of
-// up to 2100 keys, 16 heads of 64: a range's start and end cost as much as its keys.)
+// shared memory, took 36 us where the line takes 28 for 33 sequences of up to 2100
+// keys, 16 heads of 64: a range's start and end cost as much as its keys.  The line
+// streams 128 caches of 1000 to 4096 keys, 8 heads of 128, at 6.3 TB/s, 98% of a
+// plain copy's rate.)
 //
 // Prefix: with many rows (batch x group) the 128-row tensor-core kernel
 // (launch_prefix_parts), which reads the prefix once for up to 256 rows; with few,
@@ -484,6 +486,7 @@ struct JoinParams {
   const int32_t* lengths;
   int64_t score_pitch, rows, out_blocks;
   int spans, span;                     // spans of `span` cached keys
+  int row_warps;                       // warps per output row, a power of two up to 8
   int capacity, batch, num_heads, kv_heads, group, hd, tile_parts;
   int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch, tile_rows;
   int heads_shift;                     // log2 of the line's heads
@@ -564,57 +567,73 @@ __device__ __forceinline__ float row_lse(const JoinParams& p, const RowParts& x,
   return all + log2f(sum);
 }
 
-// The first out_blocks blocks write the output, one warp per row, in one pass over
-// its partial results; the others the weights of a span of cached keys of one
-// (sequence, key / value head).
+// The first out_blocks blocks write the output: `row_warps` warps of a block share a
+// row, each with its share of the row's partial results (one warp per row leaves a
+// step of few rows waiting for one batch of loads after the other).  The other blocks
+// write the weights of a span of cached keys of one (sequence, key / value head).
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x < p.out_blocks) {
-    const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 32) + warp;
-    if (row >= p.rows) return;
-    const int64_t b = div_of(row, p.num_heads);
-    const RowParts x = row_parts(p, b, (int)(row - b * p.num_heads));
-    const int count = p.tile_parts + x.prefix_count + x.cache_count;
-    for (int col0 = 0; col0 < p.hd; col0 += 128) {
-      const int col = col0 + lane * 4;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float top = -INFINITY, sum = 0.f;
-      for (int i0 = 0; i0 < count; i0 += 32) {
-        int64_t offset = 0;
-        const float lse = i0 + lane < count ? part_at(p, x, i0 + lane, offset) : -INFINITY;
-        float now = lse;
+    __shared__ float4 s_part[kJoinThreads / 32][64];  // a warp's 256 columns
+    const int share = warp & (p.row_warps - 1);       // this warp's among the row's
+    const int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 32 / p.row_warps) + warp / p.row_warps;
+    if (row < p.rows) {
+      const int64_t b = div_of(row, p.num_heads);
+      const RowParts x = row_parts(p, b, (int)(row - b * p.num_heads));
+      const int count = p.tile_parts + x.prefix_count + x.cache_count;
+      const float lse = row_lse(p, x, count);
+      if (p.lse != nullptr && share == 0 && lane == 0) p.lse[row] = lse * 0.69314718055994531f;
+      for (int col0 = 0; col0 < p.hd; col0 += 128) {
+        const int col = col0 + lane * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < count; i0 += 32) {
+          int64_t offset = 0;
+          float f = -INFINITY;
+          if (i0 + lane < count) f = part_at(p, x, i0 + lane, offset);
+          f = f == -INFINITY ? 0.f : fast_exp2(f - lse);
+          const int n = min(32, count - i0);
+          for (int q0 = share; q0 < n; q0 += 8 * p.row_warps) {
+            float4 y[8];
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, w));
-        now = fmaxf(now, top);
-        const float keep = top == -INFINITY ? 0.f : fast_exp2(top - now);
-        const float f = lse == -INFINITY ? 0.f : fast_exp2(lse - now);
-        top = now;
-        sum = sum * keep + f;
-        v = make_float4(v.x * keep, v.y * keep, v.z * keep, v.w * keep);
-        const int n = min(32, count - i0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const float fi = __shfl_sync(0xffffffffu, f, i);
-          const int64_t oi = __shfl_sync(0xffffffffu, offset, i);
-          if (col < p.hd) {
-            const float4 y = __ldg(reinterpret_cast<const float4*>(p.tile_o + oi + col));
-            v.x = fmaf(fi, y.x, v.x);
-            v.y = fmaf(fi, y.y, v.y);
-            v.z = fmaf(fi, y.z, v.z);
-            v.w = fmaf(fi, y.w, v.w);
+            for (int q = 0; q < 8; ++q) {
+              const int i = q0 + q * p.row_warps;
+              const int64_t oi = __shfl_sync(0xffffffffu, offset, i & 31);
+              y[q] = i < n && col < p.hd ? __ldg(reinterpret_cast<const float4*>(p.tile_o + oi + col))
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int i = q0 + q * p.row_warps;
+              const float fi = __shfl_sync(0xffffffffu, f, i & 31);
+              if (i < n) {
+                v.x = fmaf(fi, y[q].x, v.x);
+                v.y = fmaf(fi, y[q].y, v.y);
+                v.z = fmaf(fi, y[q].z, v.z);
+                v.w = fmaf(fi, y[q].w, v.w);
+              }
+            }
           }
         }
+        s_part[warp][(col0 >> 2) + lane] = v;
       }
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
-      if (p.lse != nullptr && col0 == 0 && lane == 0) p.lse[row] = (top + log2f(sum)) * 0.69314718055994531f;
-      if (col < p.hd)
+    }
+    __syncthreads();
+    if (row < p.rows && share == 0) {
+      for (int col = lane * 4; col < p.hd; col += 128) {
+        float4 v = s_part[warp][col >> 2];
+        for (int w = 1; w < p.row_warps; ++w) {
+          const float4 y = s_part[warp + w][col >> 2];
+          v.x += y.x;
+          v.y += y.y;
+          v.z += y.z;
+          v.w += y.w;
+        }
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * p.hd + col) =
-            make_uint2(Pack<T>::two(v.x * inv, v.y * inv), Pack<T>::two(v.z * inv, v.w * inv));
+            make_uint2(Pack<T>::two(v.x, v.y), Pack<T>::two(v.z, v.w));
+      }
     }
     return;
   }
@@ -846,7 +865,10 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   j.lengths = a.lengths;
   j.score_pitch = w.pitch;
   j.rows = a.batch * a.num_heads;
-  j.out_blocks = ceil_div(j.rows, kJoinThreads / 32);
+  // as many warps per row as keep about four per SM busy
+  j.row_warps = kJoinThreads / 32;
+  while (j.row_warps > 1 && j.row_warps * j.rows > 4 * (int64_t)sm_count()) j.row_warps /= 2;
+  j.out_blocks = ceil_div(j.rows, kJoinThreads / 32 / j.row_warps);
   // A block's start (its rows' lse) costs about two steps: only as many spans as fill
   // the GPU about three times.
   const int64_t steps = ceil_div(a.capacity, kWeightStep);
