@@ -381,8 +381,8 @@ typedef struct ttj_prompt_attn_args {
  * out[t,h] = sum over the tokens u <= t of t's own prompt of p[t,u] v[u, h/group],
  * p[t,:] = softmax(scale * q[t,h] . k[u, h/group]).  fp32 statistics; the
  * probabilities are rounded to `dtype` for the product with v, as in
- * ttj_flash_attn_fwd.  Tokens of other prompts are not read into a row's
- * result whatever they hold (infinities and NaN included).
+ * ttj_flash_attn_fwd.  Tokens that a row does not attend (other prompts', later
+ * ones) stay out of its result whatever they hold, infinities and NaN included.
  */
 int ttj_prompt_attn_fwd(const ttj_prompt_attn_args* args, ttj_stream_t stream);
 

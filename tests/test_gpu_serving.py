@@ -70,6 +70,33 @@ def test_other_prompts_contents_never_matter(dt, lens, Hq, Hkv, hd):
     assert torch.equal(dirty[first + lens[1]:], clean[first + lens[1]:])
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,hd", [(2, 2, 64), (4, 1, 64), (7, 1, 40), (4, 2, 128), (6, 2, 96), (2, 1, 256)])
+@pytest.mark.parametrize("what,bad", [("v", math.nan), ("v", -math.inf), ("k", math.nan), ("kv", math.nan)])
+def test_later_tokens_of_the_prompt_never_matter(dt, Hq, Hkv, hd, what, bad):
+    """An infinity or NaN in a token's key or value reaches the rows from that token on
+    and no earlier one (which meet it only behind the causal mask)."""
+    lens, tokens = [300, 70, 129], (17, 130, 255, 298)
+    q, k, v = (t.clone() for t in prompt_case(lens, Hq, Hkv, hd, DT[dt], 17))
+    plan = ops.PromptPlan(lens, Hq, Hkv, hd, q.device)
+    for t in tokens:
+        dirty_k, dirty_v = k.clone(), v.clone()
+        if "k" in what:
+            dirty_k[t] = bad
+        if "v" in what:
+            dirty_v[t, :, 3] = bad
+        out = ops.prompt_attn(q, dirty_k, dirty_v, plan)
+        ref, _, bound = prompt_ref(q[:t], k[:t], v[:t], [t], hd ** -0.5)
+        check(out[:t], ref, bound, t)
+        hit = out[t:300].float()
+        if what == "v":
+            assert not bool(torch.isfinite(hit[..., 3]).any()) and bool(torch.isfinite(hit[..., :3]).all())
+        else:
+            assert bool(torch.isnan(hit).all())
+        assert bool(torch.isfinite(out[300:].float()).all())
+    ops.check_device_status(q.device)
+
+
 @pytest.mark.parametrize("hd,g", [(64, 1), (64, 4), (128, 2), (256, 1)])
 def test_prompt_attn_is_one_prompt_at_a_time(hd, g):
     """Packing changes nothing: each prompt alone gives the same rows."""

@@ -24,7 +24,10 @@
 // the tensor) can sit in its last K/V tile and hold anything: their scores are
 // replaced by -inf before any arithmetic, and P.V reads V only up to the last
 // visible key rounded up to 16 rows, the rounding's rows zeroed in shared memory
-// (0 * NaN would not be 0).
+// (0 * NaN would not be 0).  Later tokens of the row's own prompt do meet P = 0 in
+// the tiles on the diagonal: a row that comes out NaN although its softmax is finite
+// and such a token holds an infinity or NaN is computed again from its own keys
+// alone (repair_row; rows that need no repair pay one multiply-add per output).
 //
 // Roles, tensor-memory layouts and schedules are those of the dense kernel
 // (flash_attn_sm100.cu), whose measurements chose them:
@@ -65,6 +68,8 @@ struct GroupedParams {
   int batch, prefix, split_keys, row_items;  // prefix: row_items = ceil(B / (tiles * positions))
   float scale_log2;
   int* status;
+  const void *q, *k, *v;  // prompts: for repair_row
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
 };
 
 template <int HD>
@@ -212,6 +217,81 @@ __device__ __forceinline__ void store_box(uint32_t box, int64_t at, int r0, int 
 __device__ __forceinline__ void box_free() {
   if ((threadIdx.x & 31) == 0) bulk_wait_group_read<0>();
   __syncwarp();
+}
+
+// Output row `at` of head `head` and token q_row again, by one warp, from the keys
+// k0 .. k0 + limit alone, if a key beyond (before k0 + end) that its tiles multiplied
+// by P = 0 holds an infinity or NaN.  Lane l has dimensions 8 l .. 8 l + 7.
+template <typename T>
+__device__ __noinline__ void repair_row(const GroupedParams& p, int64_t q_row, int head, int kvh, int64_t k0, int limit,
+                                        int end, int64_t at) {
+  const int lane = threadIdx.x & 31;
+  const bool live = lane * 8 < p.hd;
+  const T* kp = static_cast<const T*>(p.k) + k0 * p.k_row + kvh * p.k_head + lane * 8;
+  const T* vp = static_cast<const T*>(p.v) + k0 * p.v_row + kvh * p.v_head + lane * 8;
+  auto load = [&](const T* from, float (&x)[8]) {
+    const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = Pack<T>::unpack(ws[j]);
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    }
+  };
+  float x[8], q[8], o[8] = {};
+  bool found = false;
+  for (int u = limit + 1; u < end && !found; ++u) {
+    load(vp + u * p.v_row, x);
+    float z = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z = fmaf(x[j], 0.f, z);
+    found = __any_sync(0xffffffffu, z != 0.f);  // NaN from an infinity or NaN
+  }
+  if (!found) return;
+  load(static_cast<const T*>(p.q) + q_row * p.q_row + head * p.q_head + lane * 8, q);
+  float m = -INFINITY, l = 0.f;
+  for (int u = 0; u <= limit; ++u) {
+    load(kp + u * p.k_row, x);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(q[j], x[j], s);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    s *= p.scale_log2;
+    const float mn = fmaxf(m, s);
+    const float keep = m == -INFINITY ? 0.f : fast_exp2(m - mn), e = mn == -INFINITY ? 0.f : fast_exp2(s - mn);
+    l = l * keep + e;
+    m = mn;
+    load(vp + u * p.v_row, x);
+    bool all = true;  // every output is NaN already: it stays so
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o[j] = fmaf(e, x[j], o[j] * keep);
+      all = all && o[j] != o[j];
+    }
+    if ((u & 63) == 63 && __all_sync(0xffffffffu, all || !live)) break;
+  }
+  if (!live) return;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = Pack<T>::two(o[2 * j] / l, o[2 * j + 1] / l);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.hd + lane * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The rows of a softmax warp (from tile row r0) whose bit is set in `rows`.
+template <typename T>
+__device__ __forceinline__ void repair_rows(uint32_t rows, int r0, int t, int keys, const Seg& s, const GroupedParams& p) {
+  if ((threadIdx.x & 31) == 0) bulk_wait_group_all();  // the rows' first stores are done
+  __syncwarp();
+  for (; rows != 0u; rows &= rows - 1u) {
+    const int r = r0 + __ffs(rows) - 1, pos = row_pos(r, p);
+    const int64_t at = row_index(r, pos, t, s, p);
+    if (at < 0) continue;
+    const int end = min((keys + 15) & ~15, s.nk);  // P.V reads V up to here
+    repair_row<T>(p, s.q0 + t * p.positions + pos, s.kvh * p.group + r - pos * p.group, s.kvh, s.k0,
+                  row_limit<false>(pos, t, s, p), end, at);
+  }
 }
 
 // Softmax, two warps per tile and TMEM lane quarter (head_dim 64): warp w serves
@@ -392,6 +472,26 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
         st_shared_u32(box + (g + 8) * 128 + ((n ^ (g & 7)) << 4) + 4 * kq, wb);
       }
       store_box<T, 16>(box, row_index(r0 + (lane & 15), pos3 >> 16, t, s, p), r0, t, 0, s, tm_out, p);
+      uint64_t za = 0ull, zb = 0ull;  // NaN where a row's output is (or infinite)
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        za = ffma2(f2_pack(__uint_as_float(o[4 * n]), __uint_as_float(o[4 * n + 1])), 0ull, za);
+        zb = ffma2(f2_pack(__uint_as_float(o[4 * n + 2]), __uint_as_float(o[4 * n + 3])), 0ull, zb);
+      }
+      float a0, a1, b0, b1;
+      f2_unpack(za, a0, a1);
+      f2_unpack(zb, b0, b1);
+      uint32_t bad_a = __ballot_sync(0xffffffffu, a0 + a1 != 0.f && l_a - l_a == 0.f);
+      uint32_t bad_b = __ballot_sync(0xffffffffu, b0 + b1 != 0.f && l_b - l_b == 0.f);
+      if ((bad_a | bad_b) != 0u) {
+        uint32_t rows = 0u;  // four lanes per row
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          rows |= ((bad_a >> (4 * i)) & 15u) != 0u ? 1u << i : 0u;
+          rows |= ((bad_b >> (4 * i)) & 15u) != 0u ? 256u << i : 0u;
+        }
+        repair_rows<T>(rows, r0, t, tile_keys<PREFIX>(s, t, p.positions), s, p);
+      }
     }
     // The next item's first P.V overwrites O_t only after this thread's next
     // p_full arrival, which follows these TMEM loads.
@@ -539,12 +639,16 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint32_t tm
       // (Staging 64 columns in shared memory for a TMA box took ~2300 cycles of an
       // item's ~7000 with one key tile: two proxy fences and a wait for the box.)
       T* out = static_cast<T*>(p.out) + at * p.hd;
+      uint64_t z = 0ull;  // NaN where the row's output is (or infinite)
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         if (32 * c >= p.hd) break;  // uniform
         uint32_t o[32];
         __syncwarp();  // (rows of no position stored nothing in the last round)
         tmem_ld32(t_o + c * 32, o);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          z = ffma2(f2_pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])), 0ull, z);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           if (at < 0) break;
@@ -561,6 +665,10 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint32_t tm
           }
         }
       }
+      float z0, z1;
+      f2_unpack(z, z0, z1);
+      const uint32_t bad = __ballot_sync(0xffffffffu, at >= 0 && z0 + z1 != 0.f && l_run - l_run == 0.f);
+      if (bad != 0u) repair_rows<T>(bad, r0, t, keys, sg, p);
     }
   }
 }
@@ -569,7 +677,7 @@ template <typename T, int HD, bool PREFIX>
 __global__ void __launch_bounds__(GroupedSmem<HD>::kThreads, 1)
 grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
-                    const GroupedParams p) {
+                    const __grid_constant__ GroupedParams p) {
   using L = GroupedSmem<HD>;
   constexpr int SK = L::kStagesK, SV = L::kStagesV;
   constexpr int NT = L::kNT;
@@ -1063,6 +1171,12 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
   p.wide_store = p.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   p.status = a.status;
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.q_row = a.q_token_stride, p.q_head = a.q_head_stride;
+  p.k_row = a.k_token_stride, p.k_head = a.k_head_stride;
+  p.v_row = a.v_token_stride, p.v_head = a.v_head_stride;
   return dispatch<false>(a.dtype, x, p, sm_count(), stream);
 }
 
