@@ -20,7 +20,8 @@
 //    search, and a fourth resident block, measured 0 to 5% slower.)
 // 2. Copying (bound by the kept rows' bytes): a warp takes 32 output rows in the
 //    order of the output's memory and copies K and V rows in 16-byte pieces, eight
-//    rows in flight.
+//    rows in flight: 173 us for 64 caches cut to 2048 rows of 8 heads of 128, 6.2
+//    TB/s of the 6.45 of a plain copy.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -37,7 +38,9 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarpsPerBlock = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBlockKeys = 4096;         // rows per block that a cluster is sized for
+// rows per block that a cluster is sized for: 8192 measures within 1% of 4096, 2048 up
+// to 19% slower (8 caches of 16384 rows, 8 heads: 73 us, 87 with 2048)
+constexpr int kBlockKeys = 4096;
 constexpr int kMaxKeysPerThread = 20;    // held in registers; longer slices are re-read
 constexpr int kList = 2 * kThreads;      // keys that the search ends on
 static_assert(32 * kMaxKeysPerThread < 1024, "a warp's three counts share one word");

@@ -18,7 +18,10 @@
 // tiles A and B that share every K/V tile (head_dim above 128: one tile), or, for
 // the prefix, (head, 2 P sequences, a range of the prefix's keys), whose partial
 // result (o, log2 of the sum) a later kernel joins.  One persistent CTA per SM,
-// items dealt longest first in snake order.
+// items dealt longest first, all heads of an entry together, in snake order.  (A head's
+// entries together, the dense kernel's order when K and V exceed the L2, measured 2 to
+// 28% slower on ten batches of 65 to 540 MB of K and V, and 5 and 8% faster on two of
+// 2 and 4 prompts of 65536 and 32768 tokens, 8 heads of 128.)
 //
 // Keys that no row of an item may see (later tokens, the next prompt's, rows past
 // the tensor) can sit in its last K/V tile and hold anything: their scores are
@@ -39,6 +42,13 @@
 //   warps 4..    softmax: head_dim 64, 8 warps per tile with 16 rows each, P in its
 //                own TMEM columns; above, 4 warps per tile with 32 rows each, P
 //                written over S
+//
+// Bound by (16384 + 2049 tokens, 32 heads over 4 of 128: 2.07 ms, 1.08 PFLOP/s; 8 ragged
+// prompts of up to 2048, 16 heads of 64: 83 us, 0.56 PFLOP/s): at head_dim 128 a step
+// of two tiles takes ~3800 cycles, softmax 2050 plus its products and their hand-offs
+// 1740 per tile, alternating, against 2048 of the tensor pipe; at 64 the exponential
+// unit (60% busy) and the hand-offs.  Items of one or two key tiles (96 prompts of up
+// to 256 tokens: 67 us, 3.6 TB/s) take ~5 us each, their chain of barriers.
 #include <atomic>
 
 #include "attn_math.cuh"
@@ -51,7 +61,6 @@ namespace {
 constexpr int kTile = 128;                  // rows of a query tile, keys of a K/V tile
 constexpr int kChunkBytes = 128 * 128;      // [128 rows][64 columns] of 16-bit, swizzled
 constexpr uint32_t kTmemCols = 512;
-constexpr int64_t kHeadMajorKvBytes = int64_t(96) << 20;
 
 struct GroupedParams {
   void* out;              // prompts: [T, Hq, hd]
@@ -61,7 +70,6 @@ struct GroupedParams {
   float* part_lse;        // prefix: [splits][B][Hq], log2 of the sum of exponentials
   int num_items, num_entries, kv_heads, group, positions;  // positions = 128 / group
   int num_heads, hd;
-  int head_major;         // item order: 1 = a head's entries consecutive
   int kv_shift;           // log2 of kv_heads, or -1
   int box_store;          // head_dim 64: a softmax warp's rows are whole groups, its output a TMA box
   int wide_store;         // head_dim above: output rows are 32-byte aligned
@@ -124,14 +132,8 @@ __device__ __forceinline__ Seg seg_of(int item, const GroupedParams& p) {
     s.nk = min(p.split_keys, p.prefix - s.k0);
     s.rel = 0;
   } else {
-    int e;
-    if (p.head_major) {
-      s.kvh = item / p.num_entries;
-      e = item - s.kvh * p.num_entries;
-    } else {
-      e = p.kv_shift >= 0 ? item >> p.kv_shift : item / p.kv_heads;
-      s.kvh = item - e * p.kv_heads;
-    }
+    const int e = p.kv_shift >= 0 ? item >> p.kv_shift : item / p.kv_heads;
+    s.kvh = item - e * p.kv_heads;
     const int4 w = __ldg(p.plan + e);
     s.q0 = w.x;
     s.nq = w.y;
@@ -1163,9 +1165,6 @@ int launch_prompt_attn(const ttj_prompt_attn_args& a, cudaStream_t stream) {
   p.group = (int)(a.num_heads / a.num_kv_heads);
   p.positions = kTile / p.group;
   p.hd = (int)a.head_dim;
-  // As in the dense kernel: when all heads' K and V exceed about 3/4 of the L2,
-  // a head's items run consecutively and share its K/V there.
-  p.head_major = a.tokens * a.num_kv_heads * a.head_dim * 4 > kHeadMajorKvBytes ? 1 : 0;
   p.kv_shift = (p.kv_heads & (p.kv_heads - 1)) == 0 ? __builtin_ctz((unsigned)p.kv_heads) : -1;
   p.box_store = p.hd <= 64 && 16 % p.group == 0;
   p.wide_store = p.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;

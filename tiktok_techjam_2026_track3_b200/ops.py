@@ -455,7 +455,7 @@ def _group(num_heads: int, num_kv_heads: int) -> int:
 class PromptPlan:
     """Work plan of a packed batch of prompts: built once from the prompts' lengths
     (on the host, zero lengths allowed) and read by every layer's ``prompt_attn``.
-    The copy to the device is ordered on the stream current at construction."""
+    Its table is on the device when the constructor returns, for any stream."""
 
     def __init__(self, seq_lens: Union[Sequence[int], torch.Tensor], num_heads: int, num_kv_heads: int,
                  head_dim: int, device: Union[torch.device, str, int]) -> None:
