@@ -126,8 +126,8 @@ _FORMATS = {vp: "P", i64: "q", ci: "i", C.c_float: "f", C.c_size_t: "N"}
 
 
 class PackedCall:
-    """An entry point ``int f(const args*, stream)`` called with its struct's fields
-    as positional values: one ``struct`` packing instead of a ctypes assignment per
+    """An entry point ``int f(const args*, stream)`` called with a tuple of its struct's
+    field values: one ``struct`` packing instead of a ctypes assignment per
     field (about 5 us less for 30 fields).  NULL pointers are 0."""
 
     def __init__(self, name: str, args: type) -> None:
@@ -136,7 +136,7 @@ class PackedCall:
         self._pack = struct.Struct("@" + "".join(_FORMATS[t] for _, t in args._fields_) + "0P").pack
         self._fn = None
 
-    def __call__(self, stream: int, *values) -> None:
+    def __call__(self, stream: int, values: tuple) -> None:
         fn = self._fn
         if fn is None:
             fn = load()[self.name]  # a function object of its own, with its own argument types

@@ -406,12 +406,10 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 # ------------------------------------------------------- serving: prompts, caches
 
-def _strided(t: torch.Tensor, name: str) -> Tuple:
+def _strided(t: torch.Tensor) -> Tuple:
     """(t, address, element strides of all dimensions but the last): views whose rows
     are contiguous and 16-byte aligned are read in place, anything else is copied."""
     st, p = t.stride(), t.data_ptr()
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (got {t.device}); there is no CPU path")
     if len(st) == 3:
         a, b, c = st
         if c == 1 and a > 0 and b > 0 and not (a | b) & 7 and not p & 15:
@@ -429,21 +427,34 @@ def _strided(t: torch.Tensor, name: str) -> Tuple:
     return (t, t.data_ptr(), *(s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1])))
 
 
-def _same(ref: torch.Tensor, **tensors: torch.Tensor) -> None:
-    dtype, device = ref.dtype, ref.device
-    for name, t in tensors.items():
-        if t.dtype != dtype or t.device != device:
-            raise RuntimeError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
-
-
-def _launch(call: _lib.PackedCall, device: torch.device, *values) -> None:
-    """Enqueue on `device`'s current stream, with that device current."""
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        call(torch._C._cuda_getCurrentRawStream(index), *values)
+def _same(ref: torch.Tensor, names: Tuple[str, ...], *tensors: torch.Tensor) -> None:
+    """`ref` is on a GPU and `tensors` share its dtype and device."""
+    dtype, device = ref.dtype, ref.get_device()
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != device or device < 0:
+            break
     else:
-        with torch.cuda.device(device):
-            call(torch._C._cuda_getCurrentRawStream(index), *values)
+        return
+    for name, t in zip(("the first operand",) + names, (ref,) + tensors):
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor (got {t.device}); there is no CPU path")
+        if t.dtype != dtype or t.device != ref.device:
+            raise RuntimeError(f"{name} must be {dtype} on {ref.device}, got {t.dtype} on {t.device}")
+
+
+def _launch(call: _lib.PackedCall, index: int, *values) -> None:
+    """Enqueue on device `index`'s current stream, with that device current."""
+    if torch._C._cuda_getDevice() == index:
+        call(torch._C._cuda_getCurrentRawStream(index), values)
+    else:
+        with torch.cuda.device(index):
+            call(torch._C._cuda_getCurrentRawStream(index), values)
+
+
+def _status(index: int) -> int:
+    """Address of device `index`'s status word."""
+    w = _status_words.get(index)
+    return (status_word(torch.device("cuda", index)) if w is None else w).data_ptr()
 
 
 def _group(num_heads: int, num_kv_heads: int) -> int:
@@ -496,20 +507,20 @@ def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PromptP
         for t, n, want in ((q, "q", plan.q_shape), (k, "k", plan.kv_shape), (v, "v", plan.kv_shape)):
             if t.shape != want:
                 raise RuntimeError(f"{n} must be {list(want)} for this plan, got {list(t.shape)}")
-    _same(q, k=k, v=v)
-    q, qp, qt, qh = _strided(q, "q")
-    k, kp, kt, kh = _strided(k, "k")
-    v, vp, vt, vh = _strided(v, "v")
-    dev = q.device
-    if plan.table.device != dev:
+    _same(q, ("k", "v"), k, v)
+    q, qp, qt, qh = _strided(q)
+    k, kp, kt, kh = _strided(k)
+    v, vp, vt, vh = _strided(v)
+    dev, index = q.device, q.get_device()
+    if plan.table.get_device() != index:
         raise RuntimeError(f"the plan is on {plan.device}, q on {dev}")
     if out is None:
         out = q.new_empty(plan.q_shape)
     elif out.shape != plan.q_shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [T,Hq,hd] tensor of q's dtype on q's device")
     lse = torch.empty(plan.q_shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-    _launch(_lib.prompt_attn_fwd, dev, qp, kp, vp, out.data_ptr(), _ptr(lse) or 0, plan.table.data_ptr(),
-            plan.entries, status_word(dev).data_ptr(), plan.tokens, plan.num_heads, plan.num_kv_heads,
+    _launch(_lib.prompt_attn_fwd, index, qp, kp, vp, out.data_ptr(), _ptr(lse) or 0, plan.table.data_ptr(),
+            plan.entries, _status(index), plan.tokens, plan.num_heads, plan.num_kv_heads,
             plan.head_dim, qt, qh, kt, kh, vt, vh, plan.head_dim ** -0.5 if scale is None else float(scale), dt)
     return (out, lse) if return_lse else out
 
@@ -556,12 +567,12 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
                            (k_cache, "k_cache", own), (v_cache, "v_cache", own)):
             if t.shape != want:
                 raise RuntimeError(f"{n} must be {list(want)}, got {list(t.shape)}")
-    _same(q, prefix_k=prefix_k, prefix_v=prefix_v, k_cache=k_cache, v_cache=v_cache)
-    q, qp, qs, qh = _strided(q, "q")
-    prefix_k, pkp, pkr, pkh = _strided(prefix_k, "prefix_k")
-    prefix_v, pvp, pvr, pvh = _strided(prefix_v, "prefix_v")
-    k_cache, kp, ks, kr, kh = _strided(k_cache, "k_cache")
-    v_cache, vp, vs, vr, vh = _strided(v_cache, "v_cache")
+    _same(q, ("prefix_k", "prefix_v", "k_cache", "v_cache"), prefix_k, prefix_v, k_cache, v_cache)
+    q, qp, qs, qh = _strided(q)
+    prefix_k, pkp, pkr, pkh = _strided(prefix_k)
+    prefix_v, pvp, pvr, pvh = _strided(prefix_v)
+    k_cache, kp, ks, kr, kh = _strided(k_cache)
+    v_cache, vp, vs, vr, vh = _strided(v_cache)
     dev = q.device
     lengths = _dense(lengths, "lengths", (B,), torch.int32, dev)
     new_weights = None
@@ -573,12 +584,13 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     elif out.shape != (B, Hq, hd) or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [B,Hq,hd] tensor of q's dtype on q's device")
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    need = _decode_workspace(B, P, Cap, Hq, Hkv, hd, key_weights is not None, dev.index)
+    index = dev.index
+    need = _decode_workspace(B, P, Cap, Hq, Hkv, hd, key_weights is not None, index)
     if workspace is None or workspace.numel() * workspace.element_size() < need:
         workspace = lengths.new_empty((need // 4,))   # (a multiple of 256 bytes)
-    _launch(_lib.shared_prefix_attn_fwd, dev, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
+    _launch(_lib.shared_prefix_attn_fwd, index, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
             _ptr(new_weights) or 0, out.data_ptr(), _ptr(lse) or 0, workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), status_word(dev).data_ptr(), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
+            workspace.numel() * workspace.element_size(), _status(index), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
             hd ** -0.5 if scale is None else float(scale), dt)
     if new_weights is None and lse is None:
         return out
@@ -612,10 +624,10 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
     budget, recent = int(budget), int(recent)
     if budget <= 0 or recent < 0 or recent > budget:
         raise RuntimeError(f"budget must be positive and recent in 0 .. budget, got {budget} and {recent}")
-    _same(k_cache, v_cache=v_cache)
+    _same(k_cache, ("v_cache",), v_cache)
     dev = k_cache.device
-    k_cache, kp, ks, kr, kh = _strided(k_cache, "k_cache")
-    v_cache, vp, vs, vr, vh = _strided(v_cache, "v_cache")
+    k_cache, kp, ks, kr, kh = _strided(k_cache)
+    v_cache, vp, vs, vr, vh = _strided(v_cache)
     lengths = _dense(lengths, "lengths", (B,), torch.int32, dev)
     key_weights = _dense(key_weights, "key_weights", (B, Hkv, Cap), torch.float32, dev)
     if out is None:
@@ -627,18 +639,18 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
         kos = vos = budget * kor
     else:
         k_out, v_out = out
-        _same(k_cache, k_out=k_out, v_out=v_out)
+        _same(k_cache, ("k_out", "v_out"), k_out, v_out)
         for t, n in ((k_out, "k_out"), (v_out, "v_out")):
             if t.dim() != 4 or t.shape[0] != B or t.shape[1] < budget or t.shape[2:] != (Hkv, hd):
                 raise RuntimeError(f"{n} must be [{B}, >={budget}, {Hkv}, {hd}], got {list(t.shape)}")
-        ko, kop, kos, kor, koh = _strided(k_out, "k_out")
-        vo, vop, vos, vor, voh = _strided(v_out, "v_out")
+        ko, kop, kos, kor, koh = _strided(k_out)
+        vo, vop, vos, vor, voh = _strided(v_out)
         if ko is not k_out or vo is not v_out:
             raise RuntimeError("out must have contiguous rows and 16-byte aligned strides")
     weights = key_weights.new_empty((B, Hkv, budget))
     new_lengths = lengths.new_empty((B,))
     positions = lengths.new_empty((B, Hkv, budget))
-    _launch(_lib.cache_evict, dev, kp, vp, key_weights.data_ptr(), lengths.data_ptr(), kop, vop, weights.data_ptr(),
+    _launch(_lib.cache_evict, dev.index, kp, vp, key_weights.data_ptr(), lengths.data_ptr(), kop, vop, weights.data_ptr(),
             new_lengths.data_ptr(), positions.data_ptr(), B, Cap, Hkv, hd, budget, recent, ks, kr, kh, vs, vr, vh,
             kos, kor, koh, vos, vor, voh)
     return EvictedCache(k_out, v_out, weights, new_lengths, positions)
