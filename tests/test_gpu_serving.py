@@ -391,6 +391,24 @@ def test_evict_ties_and_special_weights():
         check_evict(k, v, w, [700, 700, 700, 699, 700], budget, recent)
 
 
+@pytest.mark.parametrize("C", [900, 4096, 9001, 40000, 90001])  # every row count per thread, clusters of 1 to 8 blocks
+def test_evict_search_ranges(C):
+    """The key that cuts lies among positive, zero or negative weights; within one value's ties; in a tiny range."""
+    g = torch.Generator().manual_seed(C)
+    H, hd, n = 2, 8, C - 3
+    k, v, _ = cache_case(6, C, H, hd, torch.float16, 1)
+    x = torch.randn(6, H, C, generator=g)
+    w = x.exp()                                                   # 0: positive over a wide range
+    w[1] = x[1].relu()                                            # half zeros
+    w[2] = x[2]                                                   # both signs
+    w[3] = -1.0 - x[3].abs()                                      # negative only
+    w[4] = torch.where(x[4] > 0, 1.0 + 2.0 ** -23, 1.0)           # two neighbouring values
+    w[5] = 7.5                                                    # one value
+    w = w.cuda()
+    for budget, recent in ((n // 7, 5), (n // 2 + n // 4, 64), (n - 1, 0), (50, 50)):
+        check_evict(k, v, w, [n] * 6, budget, recent)
+
+
 def test_evict_into_an_existing_cache_and_layouts():
     k, v, w = cache_case(3, 200, 2, 128, torch.bfloat16, 7)
     into = torch.full((3, 150, 2, 2, 128), 7.0, dtype=torch.bfloat16, device="cuda")          # k and v interleaved

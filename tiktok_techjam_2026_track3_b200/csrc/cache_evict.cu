@@ -3,21 +3,26 @@
 // 1. Choosing (weights read once, 4 bytes a row): one cluster of blocks per
 //    (sequence, key / value head), each warp a stretch of consecutive rows.  A weight
 //    compares as a 32-bit unsigned key in the order of its value, held in registers.
-//    The key `cut` of the last row to keep (the need-th largest) is bisected two
-//    bits at a time: every warp counts its keys at or above the three candidates and
-//    the counts are summed over the cluster (one barrier).  Once at most kList keys
-//    remain between cut and its next candidate, those alone are collected (in any
-//    order: only their values count) and every block bisects on from a copy.  The
-//    search ends as soon as a candidate has exactly `need` keys.  With `ties` the rows
-//    equal to the cut that stay, row i's slot is
+//    The key `cut` of the last row to keep (the need-th largest) is looked for in the
+//    range of the positive keys (or at zero, or below), cut to a quarter at a time:
+//    every warp counts its keys at or above the three candidates and the counts are
+//    summed over the cluster (one barrier).  Once at most kList keys remain in the
+//    range, those alone are collected (in any order: only their values count) and
+//    every block searches on in a copy.  The search ends as soon as a candidate has
+//    exactly `need` keys.  With `ties` the rows equal to the cut that stay, row i's
+//    slot is
 //        above(i) + min(ties, equal(i)),
 //    above / equal counting the earlier rows with a larger / an equal key: equal rows
 //    are kept lowest index first by construction.
-//    (Digit histograms in shared memory took 33 us for 512 caches of 4096 rows and
-//    81 us for 32 of 65537 where this takes 25 and 40.  A counting pass costs ~1000
-//    cycles of instruction issue per resident set of blocks, a cluster barrier as
-//    much again; blocks of 256 threads with a one-warp or an all-pairs end of the
-//    search, and a fourth resident block, measured 0 to 5% slower.)
+//    Bound by instruction issue and barriers: a counting pass takes ~1300 cycles to
+//    count, ~900 in the cluster barrier and ~700 to sum.  Weights written from their
+//    keys instead of read again saved 8.6 us of 89 for 32 caches of 65537 rows cut to
+//    8192; a start at the positive range (against all 32 bits) and a list and totals
+//    without ballots 4.7 of 80 there and 4.6 of 195 for 512 of up to 4096 cut to 2048.
+//    (Digit histograms in shared memory took 33 us for those 512 and 81 us for the 32
+//    where the first version of this took 25 and 40; blocks of 256 threads with a
+//    one-warp or an all-pairs end of the search, and a fourth resident block, measured
+//    0 to 5% slower.)
 // 2. Copying (bound by the kept rows' bytes): a warp takes 32 output rows in the
 //    order of the output's memory and copies K and V rows in 16-byte pieces, eight
 //    rows in flight: 173 us for 64 caches cut to 2048 rows of 8 heads of 128, 6.2
@@ -62,35 +67,43 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// The bits of the weight with this key, or false where several have it (NaN and
+// -infinity, the two zeros).
+__device__ __forceinline__ bool weight_of(uint32_t key, float* w) {
+  *w = __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+  return key != 0x007fffffu && key != 0x80000000u;
+}
+
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// State of the bisection: `need` keys are to be kept, `at` keys are >= cut, `above`
-// of them >= cut + 2^bits.
+// State of the search: `need` keys are to be kept, `at` keys are >= lo, `above` of
+// them >= lo + span, above < need <= at.
 struct Cut {
-  uint32_t cut;
-  int bits, at, above;
-  __device__ __forceinline__ uint32_t candidate(int q) const { return cut | ((uint32_t)q << (bits - 2)); }
+  uint32_t lo, span;
+  int at, above;
+  __device__ __forceinline__ uint32_t step() const { return (span + 3) >> 2; }
+  // n1, n2, n3 keys are >= lo + step, lo + 2 step, lo + 3 step
   __device__ __forceinline__ void take(int n1, int n2, int n3, int need) {
-    const uint32_t c1 = candidate(1), c2 = candidate(2), c3 = candidate(3);
-    if (n3 >= need) at = n3, cut = c3;
-    else if (n2 >= need) at = n2, cut = c2, above = n3;
-    else if (n1 >= need) at = n1, cut = c1, above = n2;
-    else above = n1;
-    bits -= 2;
+    const uint32_t s = step();
+    if (n3 >= need) at = n3, lo += 3 * s, span -= 3 * s;
+    else if (n2 >= need) at = n2, lo += 2 * s, span = s, above = n3;
+    else if (n1 >= need) at = n1, lo += s, span = s, above = n2;
+    else span = s, above = n1;
   }
 };
 
 // KPT: upper bound on rows per thread, held in registers; 0: any number, read from
 // memory each time.
 template <int KPT>
-__global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) choose_kernel(const ChooseParams p) {
+__global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 ? 4 : 3)) choose_kernel(const ChooseParams p) {
   // Every warp of the cluster leaves its counts with every block: [parity][block, warp].
   __shared__ uint32_t s_count[2][3][kMaxCluster * kWarpsPerBlock];
   __shared__ uint64_t s_total[kMaxCluster * kWarpsPerBlock];
+  __shared__ uint4 s_first[kWarpsPerBlock];
   __shared__ uint32_t s_list[kList];
   __shared__ int s_listed;
   cg::cluster_group cluster = cg::this_cluster();
@@ -121,6 +134,11 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
   }
   const int old = n - p.recent;              // rows below `old` compete
   const int need = p.budget - p.recent;      // for this many places
+  // the recent rows take the last slots
+  for (int i = rank * kThreads + tid; i < p.recent; i += nblocks * kThreads) {
+    w_out[need + i] = __ldg(w + old + i);
+    pos[need + i] = old + i;
+  }
   const int64_t first = (int64_t)my_warp * 32 * p.per + lane;  // rows first + 32 j
   uint32_t key[KPT > 0 ? KPT : 1];           // 0: a row that does not compete
   auto key_of = [&](int j) -> uint32_t {
@@ -131,48 +149,75 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
 #pragma unroll
     for (int j = 0; j < KPT; ++j) key[j] = j < p.per ? key_of(j) : 0u;
   }
-  // f(j, key) for this thread's rows, in order
+  // f(j, key) for this thread's rows, in order (a few keys of 0 at the end)
   auto each = [&](auto&& f) {
     if constexpr (KPT > 0) {
+      constexpr int kGroup = KPT < 4 ? KPT : 4;
 #pragma unroll
-      for (int j = 0; j < KPT; ++j)
-        if (j < p.per) f(j, key[j]);
+      for (int j0 = 0; j0 < KPT; j0 += kGroup)
+        if (j0 < p.per) {
+#pragma unroll
+          for (int j = j0; j < j0 + kGroup; ++j) f(j, key[j]);
+        }
     } else {
       for (int j = 0; j < p.per; ++j) f(j, key_of(j));
     }
   };
+  constexpr uint32_t kZero = 0x80000000u, kLowest = 0x007fffffu;  // keys of 0 and of -infinity
+  uint32_t top = 0u, low = 0xffffffffu, positive = 0u, nonnegative = 0u;
+  each([&](int, uint32_t k) {
+    top = max(top, k);
+    low = min(low, k > kZero ? k : 0xffffffffu);
+    positive += k > kZero;
+    nonnegative += k >= kZero;
+  });
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  positive = __reduce_add_sync(0xffffffffu, positive);
+  nonnegative = __reduce_add_sync(0xffffffffu, nonnegative);
+  if (lane == 0) s_first[warp] = make_uint4(top, low, positive, nonnegative);
   if (tid == 0) s_listed = 0;
   auto sync_all = [&]() {
     if (nblocks > 1) cluster.sync();
     else __syncthreads();
   };
-  sync_all();                                // every block runs: its shared memory may be written
+  sync_all();                                // every block runs: its shared memory may be used
 
   uint32_t cut = 0xffffffffu;                // need == 0: nothing competes
   int ties = 0;
   if (need > 0) {
-    Cut x{0u, 32, old, 0};
+    // Where the search starts: the positive weights' range, the zeros (which caches of
+    // rows that nothing attends hold in number), or all that is negative.
+    top = positive = nonnegative = 0u, low = 0xffffffffu;
+    for (int i = lane; i < nwarps; i += 32) {
+      const uint4 v = *cluster.map_shared_rank(&s_first[i % kWarpsPerBlock], i / kWarpsPerBlock);
+      top = max(top, v.x);
+      low = min(low, v.y);
+      positive += v.z;
+      nonnegative += v.w;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    const int n_positive = (int)__reduce_add_sync(0xffffffffu, positive);
+    const int n_nonnegative = (int)__reduce_add_sync(0xffffffffu, nonnegative);
+    Cut x = n_positive >= need      ? Cut{low, top - low + 1u, n_positive, 0}
+            : n_nonnegative >= need ? Cut{kZero, 1u, n_nonnegative, n_positive}
+                                    : Cut{kLowest, kZero - kLowest, old, n_nonnegative};
     int parity = 0;
 #pragma unroll 1
-    do {
-      const uint32_t t1 = x.candidate(1), t2 = x.candidate(2), t3 = x.candidate(3);
+    while (x.span > 1u && x.at != need && x.at - x.above > kList) {
+      const uint32_t t1 = x.lo + x.step(), t2 = t1 + x.step(), t3 = t2 + x.step();
       uint32_t c1 = 0, c2 = 0, c3 = 0;
-      if constexpr (KPT > 0) {               // (keys of 0 are below every candidate)
-#pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-          c1 += key[j] >= t1;
-          c2 += key[j] >= t2;
-          c3 += key[j] >= t3;
-        }
+      each([&](int, uint32_t k) {            // (keys of 0 are below every candidate)
+        c1 += k >= t1;
+        c2 += k >= t2;
+        c3 += k >= t3;
+      });
+      if constexpr (KPT > 0) {
         // a warp's three counts share one word
         c1 = __reduce_add_sync(0xffffffffu, c1 | c2 << 10 | c3 << 20);
         if (lane < nblocks) *cluster.map_shared_rank(&s_count[parity][0][my_warp], lane) = c1;
       } else {
-        each([&](int, uint32_t k) {
-          c1 += k >= t1;
-          c2 += k >= t2;
-          c3 += k >= t3;
-        });
         c1 = __reduce_add_sync(0xffffffffu, c1);
         c2 = __reduce_add_sync(0xffffffffu, c2);
         c3 = __reduce_add_sync(0xffffffffu, c3);
@@ -193,21 +238,24 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
       x.take((int)__reduce_add_sync(0xffffffffu, c1), (int)__reduce_add_sync(0xffffffffu, c2),
              (int)__reduce_add_sync(0xffffffffu, c3), need);
       parity ^= 1;
-    } while (x.bits > 0 && x.at != need && x.at - x.above > kList);
-    if (x.bits > 0 && x.at != need) {
-      // the keys in [cut, cut + 2^bits), collected by the first block
+    }
+    if (x.span > 1u && x.at != need) {
+      // the keys in [lo, lo + span), collected by the first block
       uint32_t* list = cluster.map_shared_rank(s_list, 0);
       int* listed = cluster.map_shared_rank(&s_listed, 0);
-      auto in_list = [&](uint32_t k) { return k != 0u && (k ^ x.cut) >> x.bits == 0u; };  // bits <= 30 here
-      int mine = 0, at = 0;
-      each([&](int, uint32_t k) { mine += __popc(__ballot_sync(0xffffffffu, in_list(k))); });
-      if (lane == 0 && mine > 0) at = atomicAdd(listed, mine);
-      at = __shfl_sync(0xffffffffu, at, 0);
+      int mine = 0;
+      each([&](int, uint32_t k) { mine += k - x.lo < x.span; });
+      int at = mine;                         // of this warp's lanes up to this one, then of those before it
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+      }
+      int base = 0;
+      if (lane == 31 && at > 0) base = atomicAdd(listed, at);
+      at += __shfl_sync(0xffffffffu, base, 31) - mine;
       each([&](int, uint32_t k) {
-        const bool in = in_list(k);
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (in) list[at + __popc(who & ((1u << lane) - 1u))] = k;
-        at += __popc(who);
+        if (k - x.lo < x.span) list[at++] = k;
       });
       sync_all();
       const int count = x.at - x.above;
@@ -215,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
       const int outside = x.above;           // keys above every listed one
 #pragma unroll 1
       do {
-        const uint32_t t1 = x.candidate(1), t2 = x.candidate(2), t3 = x.candidate(3);
+        const uint32_t t1 = x.lo + x.step(), t2 = t1 + x.step(), t3 = t2 + x.step();
         uint32_t c = ((k0 >= t1) + (k1 >= t1)) | ((k0 >= t2) + (k1 >= t2)) << 10 | ((k0 >= t3) + (k1 >= t3)) << 20;
         c = __reduce_add_sync(0xffffffffu, c);
         if (lane == 0) s_count[parity][0][warp] = c;
@@ -226,19 +274,20 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
         const uint32_t hi = __reduce_add_sync(0xffffffffu, c >> 20);
         x.take(outside + (int)(lo & 0xffffu), outside + (int)(lo >> 16), outside + (int)hi, need);
         parity ^= 1;
-      } while (x.bits > 0 && x.at != need);
+      } while (x.span > 1u && x.at != need);
     }
-    if (x.at == need) cut = x.cut - 1u;      // exactly the keys >= cut stay (cut > 0: old > need)
-    else cut = x.cut, ties = need - x.above; // every bit found: rows equal to the cut fill up
+    if (x.at == need) cut = x.lo - 1u;       // exactly the keys >= lo stay
+    else cut = x.lo, ties = need - x.above;  // the key is found: rows equal to it fill up
   }
 
   // This warp's rows above and equal to the cut, then those of the warps before it.
   uint32_t a = 0, e = 0;
-  each([&](int j, uint32_t k) {
-    const int64_t i = first + 32 * j;
-    a += __popc(__ballot_sync(0xffffffffu, i < old ? k > cut : i < n));
-    e += __popc(__ballot_sync(0xffffffffu, i < old && k == cut));
+  each([&](int, uint32_t k) {
+    a += k > cut;
+    e += k == cut;
   });
+  a = __reduce_add_sync(0xffffffffu, a);
+  e = __reduce_add_sync(0xffffffffu, e);
   if (lane < nblocks) *cluster.map_shared_rank(&s_total[my_warp], lane) = (uint64_t)a << 32 | e;
   sync_all();                                // (also: no block leaves while its list is read)
   uint64_t before = 0;
@@ -247,19 +296,29 @@ __global__ void __launch_bounds__(kThreads, KPT <= 2 ? 4 : (KPT <= 8 ? 3 : 2)) c
   a = (uint32_t)(before >> 32);
   e = (uint32_t)before;
   const uint32_t lower = (1u << lane) - 1u;
-  each([&](int j, uint32_t k) {
-    const int64_t i = first + 32 * j;
-    const bool above = i < old ? k > cut : i < n, equal = i < old && k == cut;
-    const uint32_t ab = __ballot_sync(0xffffffffu, above), eb = __ballot_sync(0xffffffffu, equal);
-    const uint32_t e_before = e + __popc(eb & lower);
-    if (above || (equal && e_before < (uint32_t)ties)) {
-      const uint32_t slot = a + __popc(ab & lower) + min((uint32_t)ties, e_before);
-      pos[slot] = (int32_t)i;
-      w_out[slot] = __ldg(w + i);
-    }
-    a += __popc(ab);
-    e += __popc(eb);
-  });
+  auto put = [&](int j, uint32_t k, uint32_t slot) {
+    const int i = (int)first + 32 * j;
+    float v;                                 // a load here would hold up the warp at every row
+    if (!weight_of(k, &v)) v = __ldg(w + i);
+    pos[slot] = i;
+    w_out[slot] = v;
+  };
+  if (ties == 0) {                           // uniform over the cluster
+    each([&](int j, uint32_t k) {
+      const uint32_t ab = __ballot_sync(0xffffffffu, k > cut);
+      if (k > cut) put(j, k, a + __popc(ab & lower));
+      a += __popc(ab);
+    });
+  } else {
+    each([&](int j, uint32_t k) {
+      const bool above = k > cut, equal = k == cut;
+      const uint32_t ab = __ballot_sync(0xffffffffu, above), eb = __ballot_sync(0xffffffffu, equal);
+      const uint32_t e_before = e + __popc(eb & lower);
+      if (above || (equal && e_before < (uint32_t)ties)) put(j, k, a + __popc(ab & lower) + min((uint32_t)ties, e_before));
+      a += __popc(ab);
+      e += __popc(eb);
+    });
+  }
 }
 
 struct CopyParams {
