@@ -43,10 +43,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarpsPerBlock = kThreads / 32;
 constexpr int kMaxCluster = 8;
-// rows per block that a cluster is sized for: 8192 measures within 1% of 4096, 2048 up
-// to 19% slower (8 caches of 16384 rows, 8 heads: 73 us, 87 with 2048)
-constexpr int kBlockKeys = 4096;
 constexpr int kMaxKeysPerThread = 20;    // held in registers; longer slices are re-read
+// rows per block that a cluster is sized for: what a block holds in registers (4096: 3%
+// slower for caches of 16384 rows, 9% of 10000, 22% of 40000; 2048: 29% for 16384)
+constexpr int kBlockKeys = kThreads * kMaxKeysPerThread;
 constexpr int kList = 2 * kThreads;      // keys that the search ends on
 static_assert(32 * kMaxKeysPerThread < 1024, "a warp's three counts share one word");
 
