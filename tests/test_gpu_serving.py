@@ -234,6 +234,22 @@ DECODES = [  # (B, P, C, Hq, Hkv, hd, lengths)
 ]
 
 
+# enough rows and prefix for the tensor-core tiles: one and several ranges and row tiles, a group wider than a tile's
+# share, every padded head_dim; the last beside its caches (a part of the SMs each)
+DECODES_TILES = [
+    (130, 513, 3, 32, 8, 128), (300, 1025, 0, 16, 16, 64), (140, 900, 5, 8, 2, 256), (40, 4099, 33, 24, 3, 80),
+    (5, 20001, 9, 128, 1, 64), (33, 26001, 40, 32, 8, 128),
+]
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,P,C,Hq,Hkv,hd", DECODES_TILES)
+def test_decode_behind_a_long_prefix(dt, B, P, C, Hq, Hkv, hd):
+    args = decode_case(B, P, C, Hq, Hkv, hd, DT[dt], B + P + C)
+    w = torch.rand(B, Hkv, C, generator=torch.Generator().manual_seed(1)).cuda()
+    check_decode(args, [(7 * i) % (C + 1) for i in range(B)], w)
+
+
 @pytest.mark.parametrize("dt", ["fp16", "bf16"])
 @pytest.mark.parametrize("B,P,C,Hq,Hkv,hd,lengths", DECODES)
 def test_decode_matches_definition(dt, B, P, C, Hq, Hkv, hd, lengths):

@@ -704,55 +704,77 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads, int64_t kv_heads, int64_t hd) {
   Cuts c{};
   const int64_t group = num_heads / kv_heads, rows = batch * group;
-  // A short prefix under few rows goes in the line, which saves a launch (512 keys, 8
-  // rows: 12.4 us a step against 14.4; 128 keys 10.9 against 14.4); beyond, the line
-  // leaves many partial results of little work each (16 rows, 4096 keys: 28.7 us
-  // against 16.4 on the tiles; 32 rows, 32768 keys: 63.8 against 25.1).
-  c.prefix_tiles = prefix > 0 && (prefix > 512 || rows > 16);
-  const int64_t tile = (c.prefix_tiles || prefix == 0 ? group : rows) <= 8 ? 8 : 16;
+  const int sms = sm_count();
+  const int64_t tile = group <= 8 ? 8 : 16;
   c.tile_rows = (int)tile;
-  c.prefix_row_tiles = prefix > 0 && !c.prefix_tiles ? (int)ceil_div(rows, tile) : 0;
   c.cache_row_tiles = (int)ceil_div(group, tile);
   c.heads = kv_heads % 4 == 0 ? 4 : (kv_heads % 2 == 0 ? 2 : 1);
-  const int64_t head_groups = kv_heads / c.heads;
+  const int64_t head_groups = kv_heads / c.heads, line_tiles = ceil_div(rows, tile);
+  // The prefix on the tensor-core tiles, in us: a key tile of a block's 256 rows takes
+  // ~1.9 and a range about two more for its start and end; its fp32 results are written
+  // and read at ~5 TB/s.  `best` ranges take the least.
+  const int64_t units = kv_heads * ceil_div(batch, plan_positions(group, hd)), tiles = ceil_div(prefix, 128);
+  auto ranges = [&](int blocks, int64_t& best) {
+    double least = 1e30;
+    best = 1;
+    for (int64_t n = 1; n <= std::min<int64_t>(tiles, 64); ++n) {
+      const int64_t per = ceil_div(tiles, n);
+      if (ceil_div(tiles, per) != n) continue;
+      const double us = 1.9 * (double)(ceil_div(units * n, blocks) * (per + 2)) +
+                        (double)(n * batch * num_heads) * (double)hd * 8e-6 / 5.;
+      if (us < least) least = us, best = n;
+    }
+    return least;
+  };
+  if (prefix > 0) {
+    // Or in the line, whose warps stream steps at ~10 TB/s from L2 (a unit's start and
+    // end costing about four) while its caches, taken as 0.4 full, come from HBM at 6.4:
+    // as long as those bound it, the prefix's steps are nearly free, and a launch and
+    // the tiles' results are saved.  (Line against tiles: 33 sequences of 16 heads of
+    // 64 behind 1001 keys 38.4 us against 43.3, 4 of 32 / 8 heads of 128 behind 2048
+    // 18.9 against 25.8, 64 behind 2048 with up to 4096 cached 117 against 129; 32
+    // behind 4096 with up to 512 43.5 against 28.8.)  Many partial results of a row
+    // cost the join ~0.02 us each.
+    const double step = 4e-6 * (double)(kv_heads * kStepKeys) * (double)hd;  // MB of K and V
+    const double cache_units = (double)(batch * c.cache_row_tiles), cache_steps = 0.4 * (double)capacity / kStepKeys;
+    const double hbm = step * (double)batch * cache_steps / 6.4;
+    const double line = step * cache_units * (capacity > 0 ? cache_steps + 4. : 0.) / 10.;
+    const double steps = (double)(line_tiles * ceil_div(prefix, kStepKeys));
+    const double workers = (double)(line_blocks_per_sm(hd) * (int64_t)sms * kWarps / c.heads);
+    const double per_worker = std::max((double)kMinSteps, (steps + cache_units * cache_steps) * (double)head_groups / workers);
+    const double more = std::max(hbm, line + step * steps / 10.) - std::max(hbm, line) +
+                        0.02 * (double)ceil_div(prefix, kStepKeys) / per_worker;
+    int64_t unused;
+    c.prefix_tiles = more > ranges(sms, unused);
+  }
+  c.prefix_row_tiles = prefix > 0 && !c.prefix_tiles ? (int)line_tiles : 0;
   c.units = head_groups * c.prefix_row_tiles + batch * head_groups * c.cache_row_tiles;
   c.pitch = c.prefix_row_tiles > 0 ? (int)tile : (int)std::min<int64_t>(group, tile);
   // As many blocks as stay resident, and no more than the longest line has work for.
   const int64_t steps = head_groups * (c.prefix_row_tiles * ceil_div(prefix, kStepKeys) +
                                        batch * c.cache_row_tiles * ceil_div(capacity, kStepKeys));
-  c.blocks = (int)std::min<int64_t>(line_blocks_per_sm(hd) * (int64_t)sm_count(),
-                                    ceil_div(steps * c.heads, kMinSteps * kWarps));
+  c.blocks = (int)std::min<int64_t>(line_blocks_per_sm(hd) * (int64_t)sms, ceil_div(steps * c.heads, kMinSteps * kWarps));
   if (!c.prefix_tiles) return c;
   // The two kernels share the GPU: the prefix's persistent blocks (one per SM) leave
   // the caches' blocks the SMs that their work is worth, by a key tile's ~1.9 us and
   // ~80 GB/s that an SM streams, caches taken as 0.6 full; as blocks of either end,
   // the line's take their place.  (Each kernel on the whole GPU in turn: 64 sequences
-  // behind 32768 keys 74 us a step, now 66; 128 over up to 4096 cached keys
-  // 267 us, now 251; with caches a third full 88 us, now 91.)  Steps of less than
-  // ~20 us in all gain nothing (33 sequences of up to 2100 keys: 47 us, shared 53).
-  const int64_t units = kv_heads * ceil_div(batch, plan_positions(group, hd)), tiles = ceil_div(prefix, 128);
+  // behind 32768 keys 69.8 us a step, now 67.8.)  Steps of less than ~20 us in all gain
+  // nothing (33 sequences of up to 2100 keys: 47 us, shared 53).
   const double prefix_us = 1.9 * (double)(units * tiles);
   const double line_us = 0.6 * 4.0 * (double)(batch * kv_heads * c.cache_row_tiles) * (double)(capacity * hd) / 80e3;
-  const int sms = sm_count();
   const int64_t want = (int64_t)(sms * prefix_us / (prefix_us + line_us) + 0.5);
   c.tile_blocks = prefix_us + line_us < 20. * sms
                       ? sms
                       : (int)std::max<int64_t>(std::min<int64_t>(want, sms), std::min(24, sms));
-  // The number of ranges with the least time, in key tiles of 128: waves x (tiles of a
-  // range + about 2 for its start and end).
   if (c.tile_blocks < sms) {
     // the line's blocks start as SMs become free: shorter stretches even out their ends
     const int64_t whole = steps * c.heads;
     c.blocks = (int)std::max<int64_t>(c.blocks, std::min<int64_t>(kShareWaves * line_blocks_per_sm(hd) * (int64_t)sms,
                                                                   whole / (kShareSteps * kWarps)));
   }
-  int64_t best = 1, best_time = INT64_MAX;
-  for (int64_t n = 1; n <= std::min<int64_t>(tiles, 64); ++n) {
-    const int64_t per = ceil_div(tiles, n);
-    if (ceil_div(tiles, per) != n) continue;
-    const int64_t time = ceil_div(units * n, c.tile_blocks) * (per + 2) * 16 + n;
-    if (time < best_time) best_time = time, best = n;
-  }
+  int64_t best;
+  ranges(c.tile_blocks, best);
   c.tile_keys = (int)(ceil_div(tiles, best) * 128);
   c.tile_parts = (int)best;
   return c;
