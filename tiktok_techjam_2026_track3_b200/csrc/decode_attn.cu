@@ -39,10 +39,11 @@ constexpr int kWarps = 4;
 constexpr int kJoinThreads = 128;
 constexpr int kWeightStep = 1024;  // cached keys per join block and step
 constexpr int kMinSteps = 2;       // of a stretch
-// Beside the prefix kernel: up to kShareWaves times as many blocks as stay resident (2
-// times 264 us for 128 caches of up to 4096 keys, 4: 261, 8: 251, 16: 260), with
-// stretches of at least kShareSteps.
-constexpr int kShareWaves = 8, kShareSteps = 8;
+// Beside the prefix kernel: up to kShareWaves times as many blocks as stay resident,
+// with stretches of at least kShareSteps (128 sequences behind 16384 keys with up to
+// 4096 cached 221 us a step, with 2 or 16 waves 221 and 234; 128 of 16 heads of 64
+// behind 8192 with up to 1000 cached 60.1, with stretches of 8 steps 67.7, 48 64.7).
+constexpr int kShareWaves = 8, kShareSteps = 24;
 
 // NR: row tiles of 8 (group heads) that a warp carries, 1 or 2.
 template <int HD, int NR>
