@@ -393,6 +393,14 @@ def test_evict_matches_definition(dt, B, C, H, hd, lengths, budget, recent):
     check_evict(*cache_case(B, C, H, hd, DT[dt], C + budget), lengths, budget, recent)
 
 
+@pytest.mark.parametrize("hd", [40, 64, 128, 200])
+def test_evict_many_caches_and_rows(hd):
+    """More kept rows than the choosing blocks copy, more caches than there are SMs; some below the budget."""
+    B, C = 40, 900
+    lengths = [(97 * b) % (C + 1) for b in range(B)]
+    check_evict(*cache_case(B, C, 4, hd, torch.bfloat16, hd), lengths, 640, 17)
+
+
 def test_evict_ties_and_special_weights():
     B, C, H, hd = 5, 700, 2, 64
     k, v, _ = cache_case(B, C, H, hd, torch.float16, 1)

@@ -1,4 +1,5 @@
-// Eviction from per-sequence caches by accumulated attention weight, two kernels.
+// Eviction from per-sequence caches by accumulated attention weight, two kernels (one
+// when few rows are kept).
 //
 // 1. Choosing (weights read once, 4 bytes a row): one cluster of blocks per
 //    (sequence, key / value head), each warp a stretch of consecutive rows.  A weight
@@ -30,7 +31,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "sm100_ptx.cuh"
 #include "ttj_internal.h"
@@ -47,6 +48,11 @@ constexpr int kMaxKeysPerThread = 20;    // held in registers; longer slices are
 // rows per block that a cluster is sized for: what a block holds in registers (4096: 3%
 // slower for caches of 16384 rows, 9% of 10000, 22% of 40000; 2048: 29% for 16384)
 constexpr int kBlockKeys = kThreads * kMaxKeysPerThread;
+// Kept rows of up to this many bytes per block are copied by the choosing blocks, which
+// saves a launch (2 caches of 256 rows cut to 128, 4 heads of 64: 8.2 us against 12.3;
+// 64 of 1000 cut to 128, 8 heads of 128, the size where it ends: 28.6 against 32.8,
+// cut to 256: 43.0 against 39.0).
+constexpr int64_t kCopyBytes = 65536;
 constexpr int kList = 2 * kThreads;      // keys that the search ends on
 static_assert(32 * kMaxKeysPerThread < 1024, "a warp's three counts share one word");
 
@@ -96,10 +102,27 @@ struct Cut {
   }
 };
 
+struct CopyParams {
+  const uint16_t *k, *v;
+  uint16_t *k_out, *v_out;
+  const int32_t* positions;  // [B][H][N]
+  int64_t rows;              // B * N * H
+  int64_t k_seq, k_row, k_head, v_seq, v_row, v_head;
+  int64_t ko_seq, ko_row, ko_head, vo_seq, vo_row, vo_head;
+  int kv_heads, budget, hd;
+};
+
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // KPT: upper bound on rows per thread, held in registers; 0: any number, read from
-// memory each time.
-template <int KPT>
-__global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 ? 4 : 3)) choose_kernel(const ChooseParams p) {
+// memory each time.  COPY: the blocks copy the kept rows of K and V, too.
+template <int KPT, bool COPY>
+__global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 && !COPY ? 4 : 3)) choose_kernel(const ChooseParams p, const CopyParams rows) {
   // Every warp of the cluster leaves its counts with every block: [parity][block, warp].
   __shared__ uint32_t s_count[2][3][kMaxCluster * kWarpsPerBlock];
   __shared__ uint64_t s_total[kMaxCluster * kWarpsPerBlock];
@@ -125,11 +148,48 @@ __global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 
     w_out[i] = 0.f;
     pos[i] = -1;
   }
+  auto sync_all = [&]() {
+    if (nblocks > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // The rows themselves, when there are few: a share of the slots per block.
+  auto copy_rows = [&]() {
+    if constexpr (!COPY) return;
+    sync_all();                              // the positions are written
+    const int shift = rows.hd <= 64 ? 3 : (rows.hd <= 128 ? 4 : 5);  // 16-byte pieces per row, rounded up
+    const int share = (p.budget + nblocks - 1) / nblocks, slot0 = rank * share;
+    const int total = max(min(share, p.budget - slot0), 0) << (shift + 1);
+    const int h = (int)(bh - b * p.kv_heads);
+    const uint16_t *k_in = rows.k + b * rows.k_seq + h * rows.k_head, *v_in = rows.v + b * rows.v_seq + h * rows.v_head;
+    uint16_t *k_to = rows.k_out + b * rows.ko_seq + h * rows.ko_head, *v_to = rows.v_out + b * rows.vo_seq + h * rows.vo_head;
+    constexpr int kUnroll = 4;
+    for (int u0 = tid; u0 < total; u0 += kUnroll * kThreads) {
+      uint4 x[kUnroll];
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int u = u0 + q * kThreads, piece = u & ((1 << shift) - 1);
+        x[q] = make_uint4(0u, 0u, 0u, 0u);
+        if (u >= total || piece * 8 >= rows.hd) continue;
+        const int64_t src = __ldcg(pos + slot0 + (u >> (shift + 1)));
+        const uint16_t* at = (u >> shift) & 1 ? v_in + src * rows.v_row : k_in + src * rows.k_row;
+        if (src >= 0) x[q] = load_once(at + piece * 8);
+      }
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int u = u0 + q * kThreads, piece = u & ((1 << shift) - 1);
+        if (u >= total || piece * 8 >= rows.hd) continue;
+        const int64_t to = slot0 + (u >> (shift + 1));
+        uint16_t* at = (u >> shift) & 1 ? v_to + to * rows.vo_row : k_to + to * rows.ko_row;
+        *reinterpret_cast<uint4*>(at + piece * 8) = x[q];
+      }
+    }
+  };
   if (n <= p.budget) {  // uniform over the cluster
     for (int i = rank * kThreads + tid; i < n; i += nblocks * kThreads) {
       w_out[i] = w[i];
       pos[i] = i;
     }
+    copy_rows();
     return;
   }
   const int old = n - p.recent;              // rows below `old` compete
@@ -177,10 +237,6 @@ __global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 
   nonnegative = __reduce_add_sync(0xffffffffu, nonnegative);
   if (lane == 0) s_first[warp] = make_uint4(top, low, positive, nonnegative);
   if (tid == 0) s_listed = 0;
-  auto sync_all = [&]() {
-    if (nblocks > 1) cluster.sync();
-    else __syncthreads();
-  };
   sync_all();                                // every block runs: its shared memory may be used
 
   uint32_t cut = 0xffffffffu;                // need == 0: nothing competes
@@ -319,23 +375,7 @@ __global__ void __launch_bounds__(kThreads, KPT == 0 || KPT > 8 ? 2 : (KPT <= 2 
       e += __popc(eb);
     });
   }
-}
-
-struct CopyParams {
-  const uint16_t *k, *v;
-  uint16_t *k_out, *v_out;
-  const int32_t* positions;  // [B][H][N]
-  int64_t rows;              // B * N * H
-  int64_t k_seq, k_row, k_head, v_seq, v_row, v_head;
-  int64_t ko_seq, ko_row, ko_head, vo_seq, vo_row, vo_head;
-  int kv_heads, budget, hd;
-};
-
-__device__ __forceinline__ uint4 load_once(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+  copy_rows();
 }
 
 // CP 16-byte pieces per row (rounded up to a power of two): 8 or 16: a warp step
@@ -396,8 +436,8 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyParams p) {
   }
 }
 
-template <int KPT>
-int launch_choose(const ChooseParams& p, int64_t caches, int cluster, cudaStream_t stream) {
+template <int KPT, bool COPY>
+int launch_choose(const ChooseParams& p, const CopyParams& rows, int64_t caches, int cluster, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(caches * cluster));
   cfg.blockDim = dim3(kThreads);
@@ -411,7 +451,7 @@ int launch_choose(const ChooseParams& p, int64_t caches, int cluster, cudaStream
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  TTJ_CUDA_TRY(cudaLaunchKernelEx(&cfg, choose_kernel<KPT>, p));
+  TTJ_CUDA_TRY(cudaLaunchKernelEx(&cfg, choose_kernel<KPT, COPY>, p, rows));
   return TTJ_OK;
 }
 
@@ -431,14 +471,16 @@ int launch_cache_evict(const ttj_cache_evict_args& a, cudaStream_t stream) {
   c.recent = (int)a.recent;
   int cluster = 1;
   while (cluster < kMaxCluster && (int64_t)cluster * kBlockKeys < a.capacity) cluster *= 2;
+  // Few caches get larger clusters where their blocks can then copy the rows (one of 8
+  // heads of 128 cut to 512 of 1000 rows: 13.7 us against 18.5).
+  const int64_t kept_bytes = a.head_dim * a.budget * 4;
+  int wide = cluster;
+  while (wide < kMaxCluster && kept_bytes > wide * kCopyBytes && caches * wide <= sm_count()) wide *= 2;
+  const bool copy = kept_bytes <= wide * kCopyBytes;
+  if (copy) cluster = wide;
   if (caches * cluster >= (int64_t)1 << 31) return fail(TTJ_ERR_UNSUPPORTED, "too many caches");
   const int64_t threads = (int64_t)cluster * kThreads;
   c.per = (int)std::max<int64_t>(1, (a.capacity + threads - 1) / threads);
-  int rc = c.per <= 2                   ? launch_choose<2>(c, caches, cluster, stream)
-           : c.per <= 8                 ? launch_choose<8>(c, caches, cluster, stream)
-           : c.per <= kMaxKeysPerThread ? launch_choose<kMaxKeysPerThread>(c, caches, cluster, stream)
-                                        : launch_choose<0>(c, caches, cluster, stream);
-  if (rc) return rc;
   CopyParams p{};
   p.k = static_cast<const uint16_t*>(a.k_cache);
   p.v = static_cast<const uint16_t*>(a.v_cache);
@@ -453,6 +495,16 @@ int launch_cache_evict(const ttj_cache_evict_args& a, cudaStream_t stream) {
   p.kv_heads = c.kv_heads;
   p.budget = c.budget;
   p.hd = (int)a.head_dim;
+  auto choose = [&](auto kpt) {
+    constexpr int n = decltype(kpt)::value;
+    return copy ? launch_choose<n, true>(c, p, caches, cluster, stream)
+                : launch_choose<n, false>(c, p, caches, cluster, stream);
+  };
+  const int rc = c.per <= 2                   ? choose(std::integral_constant<int, 2>())
+                 : c.per <= 8                 ? choose(std::integral_constant<int, 8>())
+                 : c.per <= kMaxKeysPerThread ? choose(std::integral_constant<int, kMaxKeysPerThread>())
+                                              : choose(std::integral_constant<int, 0>());
+  if (rc || copy) return rc;
   const int64_t blocks = (p.rows + 255) / 256;
   if (blocks >= (int64_t)1 << 31) return fail(TTJ_ERR_UNSUPPORTED, "too many cache rows");
   const dim3 grid((unsigned)blocks);
