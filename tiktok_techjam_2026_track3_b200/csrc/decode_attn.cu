@@ -14,12 +14,14 @@
 // zero-filled.  (One block per cache range of at most 1024 keys, joined through
 // shared memory, took 36 us where the line takes 28 for 33 sequences of up to 2100
 // keys, 16 heads of 64: a range's start and end cost as much as its keys.  The line
-// streams 128 caches of 1000 to 4096 keys, 8 heads of 128, at 6.3 TB/s, 98% of a
-// plain copy's rate.)
+// streams 128 caches of 1000 to 4096 keys, 8 heads of 128, at 6.4 TB/s, a plain copy's
+// rate, with a prefix of 2048 keys among its steps.)
 //
 // Prefix: with many rows (batch x group) the 128-row tensor-core kernel
-// (launch_prefix_parts), which reads the prefix once for up to 256 rows; with few,
-// the prefix's steps, a row tile of the batch at a time, come first in the same line.
+// (launch_prefix_parts), which reads the prefix once for up to 256 rows.  With few, or
+// with caches long enough to hide it, the prefix's steps, a row tile of the batch at a
+// time, come first in the same line: they read it from L2 while the caches' steps wait
+// for HBM (cuts_of weighs the two).
 //
 // Then one kernel joins the partial results and, with key_weights, turns the stored
 // scores into probabilities with the rows' final lse and adds them up over the group.
@@ -38,7 +40,7 @@ constexpr int kWarps = 4;
 // and 246.9 us for 128 caches of up to 4096 keys (245.2); 64 with half the step 43.5 and 248.1.
 constexpr int kJoinThreads = 128;
 constexpr int kWeightStep = 1024;  // cached keys per join block and step
-constexpr int64_t kL2Bytes = (int64_t)126 << 20;
+constexpr int64_t kL2Bytes = (int64_t)126 << 20;  // caches above it are read evict-first
 constexpr int kMinSteps = 2;       // of a stretch
 // Beside the prefix kernel: up to kShareWaves times as many blocks as stay resident,
 // with stretches of at least kShareSteps (128 sequences behind 16384 keys with up to
