@@ -794,12 +794,16 @@ Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads,
   return c;
 }
 
+// The regions start on multiples of kWorkspaceAlign, whatever the caller's base (a
+// multiple of 16 bytes): the prefix tiles store their results 32 bytes at a time.
+constexpr size_t kWorkspaceAlign = 256;
+
 struct Workspace {
   size_t tile_o, tile_lse, part_o, part_lse, before, scores, total;  // byte offsets
   int64_t pitch;                                                     // of the scores
 };
 Workspace workspace_of(const Cuts& c, int64_t batch, int64_t capacity, int64_t num_heads, int64_t hd, bool weights) {
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  auto up = [](size_t v) { return (v + kWorkspaceAlign - 1) / kWorkspaceAlign * kWorkspaceAlign; };
   const size_t rows = (size_t)batch * num_heads;
   const size_t parts = c.blocks > 0 ? (size_t)c.units * c.heads + (size_t)c.blocks * kWarps : 0;
   Workspace w;
@@ -810,7 +814,7 @@ Workspace workspace_of(const Cuts& c, int64_t batch, int64_t capacity, int64_t n
   w.part_lse = w.part_o + up(parts * c.pitch * hd * 4);
   w.before = w.part_lse + up(parts * c.pitch * 4);
   w.scores = w.before + up((size_t)(batch + 2) * 8);
-  w.total = w.scores + (weights ? up(rows * (size_t)w.pitch * 4) : 0);
+  w.total = w.scores + (weights ? up(rows * (size_t)w.pitch * 4) : 0) + kWorkspaceAlign;  // to round the base up
   return w;
 }
 
@@ -843,6 +847,7 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   const bool weights = a.key_weights != nullptr && a.capacity > 0;
   const Workspace w = workspace_of(c, a.batch, a.capacity, a.num_heads, a.head_dim, a.key_weights != nullptr);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  ws += (kWorkspaceAlign - reinterpret_cast<uintptr_t>(ws) % kWorkspaceAlign) % kWorkspaceAlign;
   float* tile_o = reinterpret_cast<float*>(ws + w.tile_o);
   float* tile_lse = reinterpret_cast<float*>(ws + w.tile_lse);
   const int64_t group = a.num_heads / a.num_kv_heads;
