@@ -49,3 +49,31 @@ def test_decode_workspace_at_any_16_byte_boundary(B, P, C, Hq, Hkv, hd, offset):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert bool((arena[:base] == 0x5A).all()) and bool((arena[base + need:] == 0x5A).all())
     ops.check_device_status(own.device)
+
+
+def test_workspaces_the_kernels_could_not_use_are_refused():
+    """Host memory and strided views: an error before any launch, from every call that takes one."""
+    args = decode_case(3, 300, 200, 8, 2, 128, torch.bfloat16, 1)
+    lens = torch.tensor([200, 0, 7], dtype=torch.int32).cuda()
+    x = torch.randn(2, 64, 256, device="cuda").half()
+    w = {n: torch.randn(s, device="cuda").half() * 0.05 for n, s in
+         (("w_qkv", (768, 256)), ("b_qkv", (768,)), ("w_o", (256, 256)), ("b_o", (256,)))}
+    block = dict(w, ln1_w=torch.ones_like(w["b_o"]), ln1_b=w["b_o"], ln2_w=torch.ones_like(w["b_o"]), ln2_b=w["b_o"],
+                 w_in=w["w_qkv"][:512].contiguous(), b_in=w["b_qkv"][:512].contiguous(),
+                 w_out=torch.randn(256, 512, device="cuda").half() * 0.05, b_out=w["b_o"])
+    q8, s8 = ops.quantize_weight(w["w_qkv"])
+    o8, so = ops.quantize_weight(w["w_o"])
+    bf = (w["b_qkv"].float(), w["b_o"].float())
+    calls = [lambda ws: ops.shared_prefix_attn(*args, lens, workspace=ws),
+             lambda ws: ops.attn_layer(x, w["w_qkv"], w["b_qkv"], w["w_o"], w["b_o"], 4, True, workspace=ws),
+             lambda ws: ops.transformer_block(x, block, 4, True, 1e-5, 1e-5, workspace=ws),
+             lambda ws: ops.int8_attn_layer(x, q8, s8, bf[0], o8, so, bf[1], 4, True, workspace=ws)]
+    n = 1 << 24
+    for call in calls:
+        want = call(None)
+        assert torch.equal(call(torch.empty(n, dtype=torch.uint8, device="cuda")), want)
+        assert torch.equal(call(torch.empty(n // 4, dtype=torch.float32, device="cuda")), want)
+        for bad in (torch.empty(n, dtype=torch.uint8), torch.empty(n, 2, dtype=torch.uint8, device="cuda")[:, 0],
+                    torch.empty(1, dtype=torch.uint8, device="cuda").expand(n)):
+            with pytest.raises(RuntimeError, match="workspace must be a contiguous tensor on cuda"):
+                call(bad)

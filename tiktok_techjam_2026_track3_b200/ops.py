@@ -61,6 +61,17 @@ def check_device_status(device: torch.device) -> None:
     _lib.check(lib.ttj_read_status(w.data_ptr(), C.byref(code), _stream(device)), "device status")
 
 
+def _workspace(workspace: Optional[torch.Tensor], need: int, device: torch.device) -> torch.Tensor:
+    """The caller's workspace if it has `need` bytes, else a fresh one.  The kernels get
+    its address alone, so one that would be used must be dense and on `device`."""
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise RuntimeError(f"workspace must be a contiguous tensor on {device}, got one on {workspace.device} "
+                           f"with strides {tuple(workspace.stride())}")
+    return workspace
+
+
 def _mask_u8(mask: Optional[torch.Tensor], b: int, s: int) -> Optional[torch.Tensor]:
     if mask is None:
         return None
@@ -188,13 +199,12 @@ def attn_layer(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: torch.Tensor, w_o: t
     if out is None:
         out = torch.empty_like(x)
     need = lib.ttj_attn_layer_workspace_size(B, S, D, dt)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    workspace = _workspace(workspace, need, x.device)
     a = _lib.AttnLayerArgs(
         x=x.data_ptr(), w_qkv=_cuda(w_qkv, "w_qkv").data_ptr(), b_qkv=_cuda(b_qkv, "b_qkv").data_ptr(),
         w_o=_cuda(w_o, "w_o").data_ptr(), b_o=_cuda(b_o, "b_o").data_ptr(),
         valid_token_mask=_ptr(km), residual=_ptr(residual), out=out.data_ptr(),
-        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(),
+        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel() * workspace.element_size(),
         status=status_word(x.device).data_ptr(), batch=B, seq_len=S, d_model=D,
         num_heads=num_heads, causal=int(bool(causal)), dtype=dt)
     _lib.check(lib.ttj_attn_layer_fwd(C.byref(a), _stream(x.device)), "ttj_attn_layer_fwd")
@@ -288,10 +298,9 @@ def transformer_block(x: torch.Tensor, params: Dict[str, torch.Tensor], num_head
     if out is None:
         out = torch.empty_like(x)
     need = lib.ttj_block_workspace_size(B, S, D, F, dt)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    workspace = _workspace(workspace, need, x.device)
     a = _lib.BlockArgs(x=x.data_ptr(), valid_token_mask=_ptr(km), out=out.data_ptr(),
-                       workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(),
+                       workspace=workspace.data_ptr(), workspace_bytes=workspace.numel() * workspace.element_size(),
                        status=status_word(x.device).data_ptr(), batch=B, seq_len=S, d_model=D,
                        num_heads=num_heads, ffn_dim=F, eps1=float(eps1), eps2=float(eps2),
                        causal=int(bool(causal)), dtype=dt, **ptrs)
@@ -375,14 +384,13 @@ def int8_attn_layer(x: torch.Tensor, w_qkv8: torch.Tensor, s_qkv: torch.Tensor,
     if out is None:
         out = torch.empty_like(x)
     need = lib.ttj_int8_attn_layer_workspace_size(B, S, D, dt)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    workspace = _workspace(workspace, need, x.device)
     a = _lib.Int8AttnLayerArgs(
         x=x.data_ptr(), w_qkv=_cuda(w_qkv8, "w_qkv").data_ptr(), s_qkv=_cuda(s_qkv, "s_qkv").data_ptr(),
         b_qkv=_cuda(b_qkv, "b_qkv").data_ptr(), w_o=_cuda(w_o8, "w_o").data_ptr(),
         s_o=_cuda(s_o, "s_o").data_ptr(), b_o=_cuda(b_o, "b_o").data_ptr(),
         valid_token_mask=_ptr(km), residual=_ptr(residual), out=out.data_ptr(),
-        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(),
+        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel() * workspace.element_size(),
         status=status_word(x.device).data_ptr(), batch=B, seq_len=S, d_model=D,
         num_heads=num_heads, causal=int(bool(causal)), dtype=dt)
     _lib.check(lib.ttj_int8_attn_layer_fwd(C.byref(a), _stream(x.device)), "ttj_int8_attn_layer_fwd")
@@ -586,11 +594,11 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     index = dev.index
     need = _decode_workspace(B, P, Cap, Hq, Hkv, hd, key_weights is not None, index)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = lengths.new_empty((need // 4,))   # (a multiple of 256 bytes)
+    workspace = _workspace(workspace, need, dev)
     _launch(_lib.shared_prefix_attn_fwd, index, qp, pkp, pvp, kp, vp, lengths.data_ptr(), _ptr(key_weights) or 0,
             _ptr(new_weights) or 0, out.data_ptr(), _ptr(lse) or 0, workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _status(index), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh, pvr, pvh, ks, kr, kh, vs, vr, vh,
+            workspace.numel() * workspace.element_size(), _status(index), B, P, Cap, Hq, Hkv, hd, qs, qh, pkr, pkh,
+            pvr, pvh, ks, kr, kh, vs, vr, vh,
             hd ** -0.5 if scale is None else float(scale), dt)
     if new_weights is None and lse is None:
         return out
