@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import DT
+from serving_ref import DT, decode_ref
 from tiktok_techjam_2026_track3_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -25,6 +25,12 @@ def decode_case(B, P, C, Hq, Hkv, hd, dtype, seed):
     gen = torch.Generator().manual_seed(seed)
     return (randn(gen, dtype, B, Hq, hd), randn(gen, dtype, P, Hkv, hd), randn(gen, dtype, P, Hkv, hd),
             randn(gen, dtype, B, C, Hkv, hd), randn(gen, dtype, B, C, Hkv, hd))
+
+
+def check(got, ref, bound, what=""):
+    err = (got.double() - ref).abs()
+    bad = ~(err <= bound)          # NaN counts as bad
+    assert not bool(bad.any()), (what, int(bad.sum()), float(err[bad].max()), float((err / bound.clamp_min(1e-30)).max()))
 
 
 # ------------------------------------------------------------------ workspaces
@@ -77,3 +83,69 @@ def test_workspaces_the_kernels_could_not_use_are_refused():
                     torch.empty(1, dtype=torch.uint8, device="cuda").expand(n)):
             with pytest.raises(RuntimeError, match="workspace must be a contiguous tensor on cuda"):
                 call(bad)
+
+
+# ------------------------------------------------------------------ scores of minus infinity
+
+# (B, P, C, Hq, Hkv, hd, lengths): the caches' line alone, with the prefix in it, and behind the prefix's tiles at
+# every padded head_dim and both row tiles (a group above 8 takes 16 rows)
+FAINT = [(2, 0, 64, 4, 2, 64, [17, 64]), (2, 40, 33, 2, 2, 128, [1, 33]), (3, 33, 20, 24, 2, 64, [1, 17, 20]),
+         (2, 130, 50, 4, 2, 256, [1, 49]), (300, 1025, 17, 16, 16, 64, [1, 17, 16] * 100),
+         (130, 513, 33, 32, 8, 128, [1, 17] * 65), (140, 900, 17, 8, 2, 256, [1, 17] * 70)]
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("where", ["last cached key", "every cached key", "every prefix key", "last prefix range",
+                                   "every key"])
+@pytest.mark.parametrize("B,P,C,Hq,Hkv,hd,lengths", FAINT)
+def test_keys_that_score_minus_infinity_weigh_nothing(dt, where, B, P, C, Hq, Hkv, hd, lengths):
+    """Such a key is as good as absent beside others, also where a partial result (a cache's or a
+    prefix range's) holds no other key; a row of such keys alone gets zeros, as one without keys."""
+    q, pk, pv, kc, vc = decode_case(B, P, C, Hq, Hkv, hd, DT[dt], P + C)
+    q[..., 5] = q[..., 5].abs() + 0.5            # times -inf: a score of -inf in every head
+    if where == "last cached key":
+        for b, n in enumerate(lengths):
+            kc[b, n - 1, :, 5] = -math.inf
+    if where in ("every cached key", "every key"):
+        kc[..., 5] = -math.inf
+    if where in ("every prefix key", "every key"):
+        pk[..., 5] = -math.inf
+    if where == "last prefix range":
+        pk[P // 2:, :, 5] = -math.inf
+    w = torch.rand(B, Hkv, C, generator=torch.Generator().manual_seed(3)).cuda()
+    lens = torch.tensor(lengths, dtype=torch.int32).cuda()
+    out, new_w, lse = ops.shared_prefix_attn(q, pk, pv, kc, vc, lens, key_weights=w, return_lse=True)
+    ref, bound, prob = decode_ref(q, pk, pv, kc, vc, lengths, hd ** -0.5)
+    assert bool(torch.isfinite(ref).all()) and bool(torch.isfinite(bound).all())
+    check(out, ref, bound)
+    want = w.double() + prob                     # fp32 scores and sums, then one fp32 addition
+    assert bool(((new_w.double() - want).abs() <= 4e-5 * prob + 2.0 ** -23 * want.abs()).all())
+    alone = where == "every key" or (where == "every cached key" and P == 0)
+    assert bool((lse == -math.inf).all()) == alone and not bool(torch.isnan(lse).any())
+    if alone:
+        assert not bool(out.any()) and torch.equal(new_w, w)
+    ops.check_device_status(q.device)
+
+
+def test_the_types_lowest_value_as_a_mask():
+    """Keys filled with the lowest bfloat16 value: their scores overflow to minus infinity."""
+    B, P, C, Hq, Hkv, hd = 130, 513, 40, 32, 8, 128
+    q, pk, pv, kc, vc = decode_case(B, P, C, Hq, Hkv, hd, torch.bfloat16, 9)
+    q = q.abs() + 1
+    lengths = [(5 * b) % (C + 1) for b in range(B)]
+    kc[:, ::2] = torch.finfo(torch.bfloat16).min
+    pk[400:] = torch.finfo(torch.bfloat16).min
+    out = ops.shared_prefix_attn(q, pk, pv, kc, vc, torch.tensor(lengths, dtype=torch.int32).cuda())
+    # the overflow is the inputs' own: in 64 bits these scores are finite and far below the others
+    ref, bound, _ = decode_ref(q, pk, pv, kc, vc, lengths, hd ** -0.5)
+    check(out, ref, bound)
+
+
+def test_an_infinite_value_of_a_key_without_weight_still_gives_nan():
+    """0 times infinity, as in the definition: the value of a key that a row attends is not masked."""
+    q, pk, pv, kc, vc = decode_case(2, 40, 33, 4, 2, 64, torch.float16, 4)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    kc[0, 0, :, 5], vc[0, 0, :, 7] = -math.inf, math.inf
+    out = ops.shared_prefix_attn(q, pk, pv, kc, vc, torch.tensor([1, 33], dtype=torch.int32).cuda())
+    assert bool(torch.isnan(out[0, :, 7]).all()) and bool(torch.isfinite(out[0, :, :7]).all())
+    assert bool(torch.isfinite(out[0, :, 8:]).all()) and bool(torch.isfinite(out[1]).all())

@@ -2,7 +2,9 @@
 //
 // The softmax over all of a row's keys splits into ranges, each giving the partial
 //   o_i = sum_u 2^(s_u - lse_i) v_u,   lse_i = log2 sum_u 2^s_u   (s = scale log2(e) q.k)
-// and joins as  o = sum_i 2^(lse_i - lse) o_i,  lse = log2 sum_i 2^lse_i.
+// and joins as  o = sum_i 2^(lse_i - lse) o_i,  lse = log2 sum_i 2^lse_i.  A range whose
+// keys all score -inf has lse_i = -inf and o_i = sum_u 0 v_u: zeros, so that its factor 0
+// leaves the others' sum as it is (and NaN where such a key's value is infinite or NaN).
 //
 // Caches: bound by their bytes, so the work is cut by bytes.  The steps (16
 // keys of one cache and head) of all caches form one line, in order; each warp of a
@@ -477,7 +479,7 @@ line_kernel(const LineParams p) {
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           if (at_row[t][e] < 0) continue;
           const int64_t row = ((at.unit + worker) * p.heads + side) * p.pitch + 8 * t + 2 * kq + e;
-          const float inv = 1.f / sum;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;  // 0: every key scores -inf
           float* out = p.part_o + row * p.hd + g;
 #pragma unroll
           for (int n = 0; n < HD / 16; ++n) {
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
     for (int r = warp; r < p.group; r += kJoinThreads / 32) {
       const RowParts y = row_parts(p, b, kvh * p.group + r);
       const float lse = row_lse(p, y, p.tile_parts + y.prefix_count + y.cache_count);
-      if (lane == 0) s_lse[r] = lse;
+      if (lane == 0) s_lse[r] = lse == -INFINITY ? INFINITY : lse;  // no key counts: no weight
     }
     __syncthreads();
   }

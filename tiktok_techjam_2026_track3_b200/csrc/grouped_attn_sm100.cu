@@ -438,7 +438,8 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
     if (!ok) break;
     l_a = row_sum4(l_a);
     l_b = row_sum4(l_b);
-    const float inv_a = 1.f / l_a, inv_b = 1.f / l_b;
+    // (of the prefix's keys all may score -inf and others count: that part is zeros)
+    const float inv_a = PREFIX && l_a == 0.f ? 0.f : 1.f / l_a, inv_b = PREFIX && l_b == 0.f ? 0.f : 1.f / l_b;
     const Seg s = seg_of<PREFIX, L::kNT>(item, p);
     float* lse = PREFIX ? p.part_lse + (int64_t)s.part * p.batch * p.num_heads : p.lse;
     if (lse != nullptr && kq < 2) {  // one thread per row
@@ -616,7 +617,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint32_t tm
     if (!mbar_wait_warp(&o_done[t], od_phase, p.status, kDevTimeoutSoftmax, abort_flag)) break;
     od_phase ^= 1u;
     tc_fence_after();
-    const float inv_l = 1.f / l_run;
+    const float inv_l = PREFIX && l_run == 0.f ? 0.f : 1.f / l_run;  // (as above: a part of zeros)
     if constexpr (PREFIX) {
       float* part = p.part_o + ((int64_t)sg.part * p.batch * p.num_heads + at) * p.hd;
 #pragma unroll 1
