@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import DT, decode_ref
+from serving_ref import DT, attend, decode_ref, out_bound
 from tiktok_techjam_2026_track3_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +149,103 @@ def test_an_infinite_value_of_a_key_without_weight_still_gives_nan():
     out = ops.shared_prefix_attn(q, pk, pv, kc, vc, torch.tensor([1, 33], dtype=torch.int32).cuda())
     assert bool(torch.isnan(out[0, :, 7]).all()) and bool(torch.isfinite(out[0, :, :7]).all())
     assert bool(torch.isfinite(out[0, :, 8:]).all()) and bool(torch.isfinite(out[1]).all())
+
+
+# ------------------------------------------------------------------ later tokens' infinities and NaN
+
+def prompt_case(lens, Hq, Hkv, hd, dtype, seed):
+    gen = torch.Generator().manual_seed(seed)
+    packed = randn(gen, dtype, sum(lens), Hq + 2 * Hkv, hd)
+    return packed[:, :Hq], packed[:, Hq:Hq + Hkv].clone(), packed[:, Hq + Hkv:].clone()
+
+
+def check_rows(out, q, k, v, first, rows):
+    """Rows `rows` of the prompt that starts at row `first` against their own keys alone in 64 bits;
+    where the definition gives an infinity or NaN, the same one."""
+    Hq, Hkv, hd = q.shape[1], k.shape[1], q.shape[2]
+    for i in rows:
+        n = slice(first, first + i + 1)
+        for h in range(Hq):
+            vh = v[n, h * Hkv // Hq]
+            ref, _, prob, spread = attend(q[first + i:first + i + 1, h], k[n, h * Hkv // Hq], vh, hd ** -0.5)
+            vmax = float(vh[torch.isfinite(vh)].abs().max())
+            got, ref = out[first + i, h].double(), ref[0]
+            ok = torch.isfinite(ref)
+            assert torch.equal(torch.isnan(got), torch.isnan(ref)), (i, h)
+            assert torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)]), (i, h)
+            bound = out_bound(q.dtype, ref, spread[0], i + 1, vmax)
+            assert bool(((got - ref).abs() <= bound)[ok].all()), (i, h, float(((got - ref).abs() / bound)[ok].max()))
+
+
+HEADS = [(2, 2, 64), (8, 2, 64), (7, 1, 40), (4, 2, 128), (6, 2, 96), (2, 1, 256), (3, 1, 200)]
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,hd", HEADS)
+def test_later_infinities_leave_long_prompts_as_they_are(dt, Hq, Hkv, hd):
+    """Single values late in a long prompt (and in a short one beside it): every row before each
+    of them keeps its result, the columns without one bit for bit."""
+    lens = [130, 9000, 60]
+    q, k, v = prompt_case(lens, Hq, Hkv, hd, DT[dt], hd)
+    plan = ops.PromptPlan(lens, Hq, Hkv, hd, q.device)
+    clean = ops.prompt_attn(q, k, v, plan)
+    bad = [(8957, 3, math.nan), (8960, 4, math.inf), (8999, 5, -math.inf), (4477, 6, math.nan)]
+    for at, col, x in bad:
+        v[130 + at, :, col] = x
+    v[100, :, 1] = math.inf
+    out = ops.prompt_attn(q, k, v, plan)
+    check_rows(out, q, k, v, 130, [4400, 4476, 4477, 4478, 8895, 8900, 8956, 8957, 8959, 8960, 8998, 8999])
+    check_rows(out, q, k, v, 0, [90, 99, 100, 129])
+    for col in range(hd):
+        hit = [at for at, c, _ in bad if c == col]
+        end = 130 + hit[0] if hit else len(out)
+        if col != 1:
+            near = slice(130 + hit[0] - 160, end) if hit else slice(0, 0)   # rows that may have been formed again
+            rest = torch.ones(len(out), dtype=torch.bool, device=out.device)
+            rest[near], rest[end:] = False, False
+            assert torch.equal(out[rest][..., col], clean[rest][..., col]), col
+            assert bool(torch.isfinite(out[:end, :, col].float()).all())
+    ops.check_device_status(q.device)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,hd", HEADS)
+def test_infinities_that_a_row_sees_meet_later_ones(dt, Hq, Hkv, hd):
+    """Columns that a row's own keys make infinite or NaN, others that only later keys do, rows
+    whose scores are NaN, and prompts without one finite column."""
+    lens = [400, 257, 300]
+    q, k, v = prompt_case(lens, Hq, Hkv, hd, DT[dt], hd + 1)
+    inf, nan = math.inf, math.nan
+    for at, col, x in [(5, 0, inf), (300, 0, nan), (7, 1, inf), (290, 1, -inf), (9, 2, -inf), (310, 2, -inf), (20, 3, nan),
+                       (305, 3, inf), (30, 4, inf), (200, 4, -inf), (320, 4, inf), (333, 5, nan), (390, 6, inf)]:
+        v[at, :, col] = x
+    k[280, :, 0] = nan                            # scores of the rows from there on
+    v[400 + 100] = inf                            # every column, more than once
+    v[400 + 250] = inf
+    v[400 + 255] = -inf
+    v[657 + 50:657 + 300:50, :, 7] = inf          # a column infinite again and again
+    k[657 + 10, :, 1] = inf                       # scores of both infinities
+    out = ops.prompt_attn(q, k, v, ops.PromptPlan(lens, Hq, Hkv, hd, q.device))
+    check_rows(out, q, k, v, 0, [0, 4, 5, 6, 8, 19, 20, 25, 199, 200, 255, 256, 270, 279])
+    assert bool(torch.isnan(out[280:400].float()).all())
+    check_rows(out, q, k, v, 400, [0, 99, 100, 200, 249, 250, 254, 255, 256])
+    check_rows(out, q, k, v, 657, [0, 9])
+    k[657 + 10, :, 1] = 0
+    out = ops.prompt_attn(q, k, v, ops.PromptPlan(lens, Hq, Hkv, hd, q.device))
+    check_rows(out, q, k, v, 657, [0, 9, 49, 50, 51, 99, 100, 128, 255, 256, 299])
+    ops.check_device_status(q.device)
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(4, 1, 64), (4, 1, 128), (2, 1, 256)])
+def test_repair_of_a_very_long_prompt_ends_no_wait(Hq, Hkv, hd):
+    """One value near the end of 200000 tokens: forming its tile's rows again takes longer than a
+    key tile's step, with other prompts' work behind it in the same blocks."""
+    n, lens = 200000, [200000] + [90] * 300
+    q, k, v = prompt_case(lens, Hq, Hkv, hd, torch.float16, 5)
+    plan = ops.PromptPlan(lens, Hq, Hkv, hd, q.device)
+    clean = ops.prompt_attn(q, k, v, plan)
+    v[n - 70, :, 2] = math.nan
+    out = ops.prompt_attn(q, k, v, plan)
+    ops.check_device_status(q.device)
+    assert torch.equal(out[n:], clean[n:]) and torch.equal(out[:n - 300], clean[:n - 300])
+    check_rows(out, q, k, v, 0, [n - 200, n - 128, n - 71, n - 70, n - 1])

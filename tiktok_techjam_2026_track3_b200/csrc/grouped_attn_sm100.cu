@@ -28,9 +28,10 @@
 // replaced by -inf before any arithmetic, and P.V reads V only up to the last
 // visible key rounded up to 16 rows, the rounding's rows zeroed in shared memory
 // (0 * NaN would not be 0).  Later tokens of the row's own prompt do meet P = 0 in
-// the tiles on the diagonal: a row that comes out NaN although its softmax is finite
-// and such a token holds an infinity or NaN is computed again from its own keys
-// alone (repair_row; rows that need no repair pay one multiply-add per output).
+// the tiles on the diagonal: an output that comes out NaN although its softmax is
+// finite and such a token holds an infinity or NaN is computed again from its row's own
+// keys alone once the block's items are done (repair_items; rows that need no repair
+// pay one multiply-add per output).
 //
 // Roles, tensor-memory layouts and schedules are those of the dense kernel
 // (flash_attn_sm100.cu), whose measurements chose them:
@@ -76,7 +77,7 @@ struct GroupedParams {
   int batch, prefix, split_keys, row_items;  // prefix: row_items = ceil(B / (tiles * positions))
   float scale_log2;
   int* status;
-  const void *q, *k, *v;  // prompts: for repair_row
+  const void *q, *k, *v;  // prompts: for repair_items
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
 };
 
@@ -221,78 +222,230 @@ __device__ __forceinline__ void box_free() {
   __syncwarp();
 }
 
-// Output row `at` of head `head` and token q_row again, by one warp, from the keys
-// k0 .. k0 + limit alone, if a key beyond (before k0 + end) that its tiles multiplied
-// by P = 0 holds an infinity or NaN.  Lane l has dimensions 8 l .. 8 l + 7.
-template <typename T>
-__device__ __noinline__ void repair_row(const GroupedParams& p, int64_t q_row, int head, int kvh, int64_t k0, int limit,
-                                        int end, int64_t at) {
-  const int lane = threadIdx.x & 31;
-  const bool live = lane * 8 < p.hd;
-  const T* kp = static_cast<const T*>(p.k) + k0 * p.k_row + kvh * p.k_head + lane * 8;
-  const T* vp = static_cast<const T*>(p.v) + k0 * p.v_row + kvh * p.v_head + lane * 8;
-  auto load = [&](const T* from, float (&x)[8]) {
-    const uint4 w = live ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = Pack<T>::unpack(ws[j]);
-      x[2 * j] = f.x;
-      x[2 * j + 1] = f.y;
-    }
-  };
-  float x[8], q[8], o[8] = {};
-  bool found = false;
-  for (int u = limit + 1; u < end && !found; ++u) {
-    load(vp + u * p.v_row, x);
-    float z = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) z = fmaf(x[j], 0.f, z);
-    found = __any_sync(0xffffffffu, z != 0.f);  // NaN from an infinity or NaN
-  }
-  if (!found) return;
-  load(static_cast<const T*>(p.q) + q_row * p.q_row + head * p.q_head + lane * 8, q);
-  float m = -INFINITY, l = 0.f;
-  for (int u = 0; u <= limit; ++u) {
-    load(kp + u * p.k_row, x);
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(q[j], x[j], s);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : fast_exp2(m - mn), e = mn == -INFINITY ? 0.f : fast_exp2(s - mn);
-    l = l * keep + e;
-    m = mn;
-    load(vp + u * p.v_row, x);
-    bool all = true;  // every output is NaN already: it stays so
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o[j] = fmaf(e, x[j], o[j] * keep);
-      all = all && o[j] != o[j];
-    }
-    if ((u & 63) == 63 && __all_sync(0xffffffffu, all || !live)) break;
-  }
-  if (!live) return;
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = Pack<T>::two(o[2 * j] / l, o[2 * j + 1] / l);
-  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at * p.hd + lane * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+// Outputs again that came out NaN or infinite only because of keys that their row does
+// not see: the tiles on the diagonal multiply those by P = 0.  Called by all softmax
+// warps of a block once its items k_lo .. k_hi are done (some of them have such a row),
+// so that no other role waits however long the prompts are; shared memory is free then.
+//
+// Column c of an output depends on column c of V alone.  Per tile and column: the first
+// key whose value is NaN, +inf, -inf (among those its products read), and the last such
+// key that some row does not see.  A row is right where it sees that last key, or is NaN
+// by keys that it sees (a NaN, infinities of both signs); infinite by those alone it is
+// that infinity, unless its own sum is not finite (which a column of finite values
+// tells); else the block forms it again, the keys dealt out over the warps.
+// (One NaN at the end of 32768 tokens, 8 heads over 2 of 128: 46 ms; one warp per row, a
+// key after the other inside the softmax loop, took 540.)
+template <int HD>
+struct Repair {
+  using L = GroupedSmem<HD>;
+  static constexpr int kThreads = L::kThreads - 128;  // every warp but the first four
+  static constexpr int kWarps = kThreads / 32;
+  static constexpr int kLanes = HD / 8;               // lanes per key, 8 dimensions each
+  static constexpr int kKeys = 32 / kLanes;           // keys of a warp's step
+  static constexpr int kParts = kWarps * kKeys;
+  static constexpr int kRows = HD == 64 ? 2 : 4;      // rows formed together (registers)
+  static constexpr int kNone = 0x7fffffff;
+  int first[3][HD], last[HD];                         // of NaN, +inf, -inf; of any
+  int rows[kTile], count;                             // to be formed again
+  float m[kParts][kRows], l[kParts][kRows], o[kParts][kRows][HD];
+};
+
+__device__ __forceinline__ void repair_sync(int threads) { asm volatile("barrier.cta.sync 1, %0;" ::"r"(threads) : "memory"); }
+__device__ __forceinline__ bool repair_any(bool mine, int threads) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(any) : "r"((uint32_t)mine), "r"(threads) : "memory");
+  return any != 0u;
 }
 
-// The rows of a softmax warp (from tile row r0) whose bit is set in `rows`.
 template <typename T>
-__device__ __forceinline__ void repair_rows(uint32_t rows, int r0, int t, int keys, const Seg& s, const GroupedParams& p) {
-  if ((threadIdx.x & 31) == 0) bulk_wait_group_all();  // the rows' first stores are done
-  __syncwarp();
-  for (; rows != 0u; rows &= rows - 1u) {
-    const int r = r0 + __ffs(rows) - 1, pos = row_pos(r, p);
-    const int64_t at = row_index(r, pos, t, s, p);
-    if (at < 0) continue;
-    const int end = min((keys + 15) & ~15, s.nk);  // P.V reads V up to here
-    repair_row<T>(p, s.q0 + t * p.positions + pos, s.kvh * p.group + r - pos * p.group, s.kvh, s.k0,
-                  row_limit<false>(pos, t, s, p), end, at);
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = Pack<T>::unpack(ws[j]);
+    x[2 * j] = f.x;
+    x[2 * j + 1] = f.y;
+  }
+}
+
+template <typename T, int HD>
+__device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x, int k_lo, int k_hi) {
+  using R = Repair<HD>;
+  constexpr int NT = GroupedSmem<HD>::kNT;
+  const int tid = threadIdx.x - 128, warp = tid >> 5, lane = tid & 31;
+  const int piece = lane % R::kLanes;                 // this lane's dimensions, 8 piece ..
+  const bool live = piece * 8 < p.hd;
+  T* const out = static_cast<T*>(p.out);
+  auto put = [&](int64_t at, int col, float v) {
+    const uint16_t w = (uint16_t)Pack<T>::two(v, 0.f);
+    *reinterpret_cast<uint16_t*>(out + at * p.hd + col) = w;
+  };
+  for (int k = k_lo; k <= k_hi; ++k) {
+    const Seg s = seg_of<false, NT>(item_of(k), p);
+    const T* const kp = static_cast<const T*>(p.k) + s.k0 * p.k_row + s.kvh * p.k_head + piece * 8;
+    const T* const vp = static_cast<const T*>(p.v) + s.k0 * p.v_row + s.kvh * p.v_head + piece * 8;
+    for (int t = 0; t < NT; ++t) {
+      const int keys = tile_keys<false>(s, t, p.positions);
+      if (keys == 0) continue;
+      const int seen = row_limit<false>(0, t, s, p) + 1;  // keys that every row sees
+      const int end = min((keys + 15) & ~15, s.nk);       // P.V reads V up to here
+      for (int i = tid; i < HD; i += R::kThreads) {
+        x.first[0][i] = x.first[1][i] = x.first[2][i] = R::kNone;
+        x.last[i] = -1;
+      }
+      if (tid == 0) x.count = 0;
+      repair_sync(R::kThreads);
+      auto scan = [&](int from, int to, bool unseen) -> bool {
+        constexpr int kStep = R::kThreads / R::kLanes, kAhead = 4;
+        bool found = false;
+        for (int u0 = from + tid / R::kLanes; u0 < to; u0 += kAhead * kStep) {
+          uint4 w[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const int64_t u = u0 + i * kStep;
+            w[i] = live && u < to ? __ldg(reinterpret_cast<const uint4*>(vp + u * p.v_row)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            float e[8], z = 0.f;
+            unpack8<T>(w[i], e);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z = fmaf(e[j], 0.f, z);
+            if (z == 0.f) continue;                       // all finite
+            found = true;
+            const int u = u0 + i * kStep;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (e[j] - e[j] == 0.f) continue;
+              int* const f = &x.first[e[j] != e[j] ? 0 : (e[j] > 0.f ? 1 : 2)][piece * 8 + j];
+              if (u < *static_cast<volatile int*>(f)) atomicMin(f, u);
+              if (unseen) atomicMax(&x.last[piece * 8 + j], u);
+            }
+          }
+        }
+        return found;
+      };
+      if (!repair_any(scan(seen, end, true), R::kThreads)) continue;
+      scan(0, seen, false);
+      repair_sync(R::kThreads);
+      for (int r = warp; r < kTile; r += R::kWarps) {     // which rows
+        const int pos = row_pos(r, p), limit = row_limit<false>(pos, t, s, p);
+        const int64_t at = row_index(r, pos, t, s, p);
+        if (at < 0) continue;
+        bool form = false, infinite = false;
+        int finite = -1;                                  // a column of finite values
+        for (int c = lane; c < p.hd; c += 32) {
+          const int f0 = x.first[0][c], f1 = x.first[1][c], f2 = x.first[2][c];
+          if (min(f0, min(f1, f2)) == R::kNone) finite = c;
+          if (x.last[c] <= limit || f0 <= limit || (f1 <= limit && f2 <= limit)) continue;
+          (f1 <= limit || f2 <= limit ? infinite : form) = true;
+        }
+        form = __any_sync(0xffffffffu, form);
+        infinite = __any_sync(0xffffffffu, infinite);
+        finite = __reduce_max_sync(0xffffffffu, finite);
+        if (form || (infinite && finite < 0)) {
+          if (lane == 0) x.rows[atomicAdd(&x.count, 1)] = r;
+        } else if (infinite) {
+          const uint16_t w = __ldcg(reinterpret_cast<const uint16_t*>(out + at * p.hd + finite));
+          const float v = Pack<T>::unpack(w).x;
+          if (v != v) continue;
+          for (int c = lane; c < p.hd; c += 32) {
+            const int f0 = x.first[0][c], f1 = x.first[1][c], f2 = x.first[2][c];
+            if (x.last[c] <= limit || f0 <= limit || (f1 <= limit) == (f2 <= limit)) continue;
+            put(at, c, f1 <= limit ? INFINITY : -INFINITY);
+          }
+        }
+      }
+      repair_sync(R::kThreads);
+      const int count = x.count;
+      for (int r0 = 0; r0 < count; r0 += R::kRows) {
+        float q[R::kRows][8], o[R::kRows][8], m[R::kRows], l[R::kRows];
+        int limit[R::kRows], most = 0;
+#pragma unroll
+        for (int i = 0; i < R::kRows; ++i) {
+          const int r = x.rows[min(r0 + i, count - 1)], pos = row_pos(r, p);
+          limit[i] = row_limit<false>(pos, t, s, p);
+          most = max(most, limit[i]);
+          const T* from = static_cast<const T*>(p.q) + (int64_t)(s.q0 + t * p.positions + pos) * p.q_row +
+                          (s.kvh * p.group + r - pos * p.group) * p.q_head + piece * 8;
+          unpack8<T>(live ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u), q[i]);
+          m[i] = -INFINITY;
+          l[i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[i][j] = 0.f;
+        }
+        uint4 kw, vw;
+        auto load = [&](int64_t u) {
+          const bool ok = live && u <= most;
+          kw = ok ? __ldg(reinterpret_cast<const uint4*>(kp + u * p.k_row)) : make_uint4(0u, 0u, 0u, 0u);
+          vw = ok ? __ldg(reinterpret_cast<const uint4*>(vp + u * p.v_row)) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        const int mine = lane / R::kLanes;
+        load(warp * R::kKeys + mine);
+        for (int u0 = warp * R::kKeys; u0 <= most; u0 += R::kParts) {
+          float ks[8], vs[8];
+          unpack8<T>(kw, ks);
+          unpack8<T>(vw, vs);
+          load((int64_t)u0 + R::kParts + mine);
+#pragma unroll
+          for (int i = 0; i < R::kRows; ++i) {
+            float c = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c = fmaf(q[i][j], ks[j], c);
+#pragma unroll
+            for (int w = R::kLanes / 2; w > 0; w >>= 1) c += __shfl_xor_sync(0xffffffffu, c, w);
+            if (u0 + mine > limit[i]) continue;
+            c *= p.scale_log2;
+            const float mn = fmaxf(m[i], c);
+            const float keep = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - mn), e = c == -INFINITY ? 0.f : fast_exp2(c - mn);
+            l[i] = fmaf(l[i], keep, e);
+            m[i] = mn;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[i][j] = fmaf(e, vs[j], o[i][j] * keep);
+          }
+        }
+        const int part = warp * R::kKeys + mine;
+#pragma unroll
+        for (int i = 0; i < R::kRows; ++i) {
+          if (piece == 0) x.m[part][i] = m[i], x.l[part][i] = l[i];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x.o[part][i][piece * 8 + j] = o[i][j];
+        }
+        repair_sync(R::kThreads);
+        for (int n = tid; n < R::kRows * HD; n += R::kThreads) {
+          const int i = n / HD, c = n % HD;
+          if (r0 + i >= count || c >= p.hd) continue;
+          const int r = x.rows[r0 + i], pos = row_pos(r, p), lim = row_limit<false>(pos, t, s, p);
+          const int f0 = x.first[0][c], f1 = x.first[1][c], f2 = x.first[2][c];
+          if (x.last[c] <= lim || f0 <= lim || (f1 <= lim && f2 <= lim)) continue;
+          float top = -INFINITY, sum = 0.f, v = 0.f;
+          for (int w = 0; w < R::kParts; ++w) top = fmaxf(top, x.m[w][i]);
+          for (int w = 0; w < R::kParts; ++w) {
+            const float f = x.m[w][i] == -INFINITY ? 0.f : fast_exp2(x.m[w][i] - top);
+            sum = x.l[w][i] == 0.f ? sum : fmaf(x.l[w][i], f, sum);
+            v = fmaf(x.o[w][i][c], f, v);
+          }
+          v /= sum;
+          if (f1 <= lim || f2 <= lim) v = sum - sum != 0.f || sum == 0.f ? NAN : (f1 <= lim ? INFINITY : -INFINITY);
+          put(row_index(r, pos, t, s, p), c, v);
+        }
+        repair_sync(R::kThreads);
+      }
+      repair_sync(R::kThreads);
+    }
+  }
+}
+
+// Item k of this block has an output that repair_items must look at (the first and the
+// last of them follow the abort flag).
+__device__ __forceinline__ void note_repair(volatile int* abort_flag, int k) {
+  if ((threadIdx.x & 31) == 0) {
+    int* const redo = const_cast<int*>(abort_flag) + 1;
+    atomicMin(&redo[0], k);
+    atomicMax(&redo[1], k);
   }
 }
 
@@ -486,15 +639,7 @@ __device__ __forceinline__ void softmax_pairs(const GroupedParams& p, uint8_t* e
       f2_unpack(zb, b0, b1);
       uint32_t bad_a = __ballot_sync(0xffffffffu, a0 + a1 != 0.f && l_a - l_a == 0.f);
       uint32_t bad_b = __ballot_sync(0xffffffffu, b0 + b1 != 0.f && l_b - l_b == 0.f);
-      if ((bad_a | bad_b) != 0u) {
-        uint32_t rows = 0u;  // four lanes per row
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          rows |= ((bad_a >> (4 * i)) & 15u) != 0u ? 1u << i : 0u;
-          rows |= ((bad_b >> (4 * i)) & 15u) != 0u ? 256u << i : 0u;
-        }
-        repair_rows<T>(rows, r0, t, tile_keys<PREFIX>(s, t, p.positions), s, p);
-      }
+      if ((bad_a | bad_b) != 0u) note_repair(abort_flag, k);
     }
     // The next item's first P.V overwrites O_t only after this thread's next
     // p_full arrival, which follows these TMEM loads.
@@ -671,7 +816,7 @@ __device__ __forceinline__ void softmax_rows(const GroupedParams& p, uint32_t tm
       float z0, z1;
       f2_unpack(z, z0, z1);
       const uint32_t bad = __ballot_sync(0xffffffffu, at >= 0 && z0 + z1 != 0.f && l_run - l_run == 0.f);
-      if (bad != 0u) repair_rows<T>(bad, r0, t, keys, sg, p);
+      if (bad != 0u) note_repair(abort_flag, k);
     }
   }
 }
@@ -709,6 +854,7 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   uint64_t* drain = o_done + 2;         // [2] per issuer: every MMA completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* redo = abort_flag + 1;  // [2] first and last of the items to repair
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -735,6 +881,8 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       mbar_init(&drain[t], 1);
     }
     *abort_flag = 0;
+    redo[0] = 0x7fffffff;
+    redo[1] = -1;
     fence_mbar_init();
   }
   if (p.positions * p.group < kTile) {
@@ -1070,6 +1218,12 @@ grouped_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       softmax_pairs<T, HD, PREFIX>(p, smem + L::kEpiOff, tmem, &tm_out, s_full, s_free, p_full, o_done, abort_flag);
     else
       softmax_rows<T, HD, PREFIX>(p, tmem, s_full, p_full, o_done, abort_flag);
+    if constexpr (!PREFIX) {
+      using R = Repair<HD>;
+      static_assert(sizeof(R) <= L::kBarOff, "the Q, K and V buffers hold it");
+      repair_sync(R::kThreads);  // every item of the block is done (or a wait ran out)
+      if (redo[0] <= redo[1] && !*abort_flag) repair_items<T, HD>(p, *reinterpret_cast<R*>(smem), redo[0], redo[1]);
+    }
   }
   tc_fence_before();
   __syncthreads();
