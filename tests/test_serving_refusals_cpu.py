@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tiktok_techjam_2026_track3_b200 import ops
+from tiktok_techjam_2026_track3_b200 import CachedAttention, ops
 
 
 def test_workspaces_that_would_be_used_are_dense_and_on_the_device():
@@ -21,3 +21,27 @@ def test_workspaces_that_would_be_used_are_dense_and_on_the_device():
     for bad in (own[::2], torch.empty(1).expand(64), torch.empty(8, 8)[:, :4]):
         with pytest.raises(RuntimeError, match="workspace must be a contiguous"):
             ops._workspace(bad, bad.numel() * 4, here)
+
+
+# ------------------------------------------------------------------ the cached attention layer
+
+@pytest.fixture
+def layer(monkeypatch):
+    """A layer whose projections run on the CPU, so that its calls reach the operators (which
+    refuse CPU tensors)."""
+    monkeypatch.setattr(ops, "linear", torch.nn.functional.linear)
+    return CachedAttention(256, 4, 2).half()
+
+
+def test_prefill_refuses_a_plan_of_other_lengths(layer):
+    """Equal totals are not enough: such a plan's rows would attend across prompts."""
+    cache = layer.new_cache(2, 16)
+    x = torch.randn(9, 256).half()
+    for other in ([5, 4], [9, 0], [4, 5, 0], [4, 4]):
+        with pytest.raises(RuntimeError, match="other prompt lengths"):
+            layer.prefill(x, [4, 5], cache, plan=layer.plan(other))
+    with pytest.raises(RuntimeError, match="9 tokens, seq_lens 8"):
+        layer.prefill(x, [4, 4], cache)
+    for lens in ([4, 5], torch.tensor([4, 5])):               # accepted up to the operator itself
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            layer.prefill(x, lens, layer.new_cache(2, 16), plan=layer.plan([4, 5]))

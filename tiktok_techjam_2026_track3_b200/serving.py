@@ -149,6 +149,12 @@ class CachedAttention(nn.Module):
         attends the prefix and its own prompt up to itself."""
         if any(cache.host_lengths):
             raise RuntimeError("prefill starts sequences: the cache must be empty")
+        lens = tuple(int(n) for n in seq_lens)
+        if x.shape[0] != sum(lens):
+            raise RuntimeError(f"x holds {x.shape[0]} tokens, seq_lens {sum(lens)}")
+        if plan is not None and plan.seq_lens != lens:
+            # (one of the same total would attend across the prompts' boundaries)
+            raise RuntimeError("the plan was built for other prompt lengths than seq_lens")
         q, k, v = self._qkv(x)
         cache.extend(seq_lens, k, v)
         plan = self.plan(seq_lens) if plan is None else plan
