@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tiktok_techjam_2026_track3_b200 import CachedAttention, ops
+from tiktok_techjam_2026_track3_b200 import CachedAttention, SharedPrefix, ops
 
 
 def test_workspaces_that_would_be_used_are_dense_and_on_the_device():
@@ -45,3 +45,36 @@ def test_prefill_refuses_a_plan_of_other_lengths(layer):
     for lens in ([4, 5], torch.tensor([4, 5])):               # accepted up to the operator itself
         with pytest.raises(RuntimeError, match="no CPU path"):
             layer.prefill(x, lens, layer.new_cache(2, 16), plan=layer.plan([4, 5]))
+
+
+def state(cache):
+    return cache.host_lengths, cache.lengths.tolist(), cache.key_weights.clone()
+
+
+def test_a_refused_prefill_leaves_the_cache_empty(layer):
+    cache = layer.new_cache(2, 16)
+    x = torch.randn(9, 256).half()
+    for args in (dict(x=x, seq_lens=[4, 5]), dict(x=x, seq_lens=[4, 5], plan=layer.plan([4, 5])),
+                 dict(x=x, seq_lens=[4, 5], prefix=SharedPrefix(x, x)), dict(x=x[:, :8], seq_lens=[4, 5])):
+        with pytest.raises(RuntimeError):
+            layer.prefill(cache=cache, **args)
+        assert cache.host_lengths == [0, 0] and cache.lengths.tolist() == [0, 0]
+
+
+def test_a_refused_decode_leaves_the_cache_as_it_was(layer, monkeypatch):
+    cache = layer.new_cache(2, 16)
+    cache.extend([3, 0], torch.randn(3, 2, 64).half(), torch.randn(3, 2, 64).half())
+    cache.key_weights[0, :, :3] = 0.5
+    before, rows = state(cache), cache.k[0, :3].clone()
+    bad = torch.zeros(4, 1, 64, dtype=torch.float16)
+    for prefix in (None, SharedPrefix(bad, bad), SharedPrefix(bad.float(), bad)):
+        with pytest.raises(RuntimeError):
+            layer.decode(torch.randn(2, 256).half(), cache, prefix)
+        now = state(cache)
+        assert now[:2] == before[:2] and torch.equal(now[2], before[2]) and torch.equal(cache.k[0, :3], rows)
+    # and where the attention is accepted but the output projection fails
+    monkeypatch.setattr(ops, "shared_prefix_attn", lambda q, *a, key_weights: (q[:, :1], key_weights + 1))
+    with pytest.raises(RuntimeError):
+        layer.decode(torch.randn(2, 256).half(), cache)
+    now = state(cache)
+    assert now[:2] == before[:2] and torch.equal(now[2], before[2])

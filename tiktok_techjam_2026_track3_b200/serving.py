@@ -82,6 +82,11 @@ class SequenceCache:
         self.lengths += 1
         self.host_lengths = [n + 1 for n in self.host_lengths]
 
+    def _drop(self) -> None:
+        """Take the last ``append`` back (rows past the lengths may hold anything)."""
+        self.lengths -= 1
+        self.host_lengths = [n - 1 for n in self.host_lengths]
+
     def evict(self, budget: int, recent: int) -> torch.Tensor:
         """Keep at most ``budget`` rows per head: the last ``recent`` and the heaviest of
         the others.  Returns the kept rows' indices [B, Hkv, budget] (-1: none)."""
@@ -155,9 +160,9 @@ class CachedAttention(nn.Module):
         if plan is not None and plan.seq_lens != lens:
             # (one of the same total would attend across the prompts' boundaries)
             raise RuntimeError("the plan was built for other prompt lengths than seq_lens")
+        cache._room(lens)
         q, k, v = self._qkv(x)
-        cache.extend(seq_lens, k, v)
-        plan = self.plan(seq_lens) if plan is None else plan
+        plan = self.plan(lens) if plan is None else plan
         ctx, lse = ops.prompt_attn(q, k, v, plan, return_lse=True)
         if prefix is not None and x.shape[0] > 0:
             # every prompt token is one more row over the prefix
@@ -165,14 +170,22 @@ class CachedAttention(nn.Module):
             none = torch.zeros(x.shape[0], dtype=torch.int32, device=x.device)
             over, lse_over = ops.shared_prefix_attn(q, prefix.k, prefix.v, no_rows, no_rows, none, return_lse=True)
             ctx = _join(ctx, lse, over, lse_over)
-        return self._out(ctx)
+        y = self._out(ctx)
+        cache.extend(lens, k, v)    # last: a refused call leaves the cache empty
+        return y
 
     def decode(self, x: torch.Tensor, cache: SequenceCache, prefix: Optional[SharedPrefix] = None) -> torch.Tensor:
         """One new token per sequence, x [B, d_model]: appended to the cache, attended, and
         the step's attention weights added to the cache's."""
         q, k, v = self._qkv(x)
         cache.append(k, v)
-        pre = self._no_prefix(k) if prefix is None else prefix
-        ctx, cache.key_weights = ops.shared_prefix_attn(q, pre.k, pre.v, cache.k, cache.v, cache.lengths,
-                                                        key_weights=cache.key_weights)
-        return self._out(ctx)
+        try:
+            pre = self._no_prefix(k) if prefix is None else prefix
+            ctx, key_weights = ops.shared_prefix_attn(q, pre.k, pre.v, cache.k, cache.v, cache.lengths,
+                                                      key_weights=cache.key_weights)
+            y = self._out(ctx)
+        except BaseException:       # a refused call leaves the cache as it was
+            cache._drop()
+            raise
+        cache.key_weights = key_weights
+        return y
