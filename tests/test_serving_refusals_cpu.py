@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tiktok_techjam_2026_track3_b200 import CachedAttention, SharedPrefix, ops
+from tiktok_techjam_2026_track3_b200 import CachedAttention, SequenceCache, SharedPrefix, ops
 
 
 def test_workspaces_that_would_be_used_are_dense_and_on_the_device():
@@ -78,3 +78,23 @@ def test_a_refused_decode_leaves_the_cache_as_it_was(layer, monkeypatch):
         layer.decode(torch.randn(2, 256).half(), cache)
     now = state(cache)
     assert now[:2] == before[:2] and torch.equal(now[2], before[2])
+
+
+def test_cache_rows_are_never_spread_over_sequences():
+    """One row for several places, other heads, another type: refused, nothing appended."""
+    cache = SequenceCache(2, 8, 2, 64, torch.float16, torch.device("cpu"))
+    row = lambda n, h=2, hd=64: torch.randn(n, h, hd).half()
+    cache.extend([1, 0], row(1), row(1))
+    for k, v in ((row(1), row(1)), (row(2), row(1)), (row(1), row(2)), (row(2, 1), row(2, 1)), (row(2, 2, 1), row(2)),
+                 (row(2), row(2).float()), (row(3), row(3))):
+        with pytest.raises(RuntimeError, match="must be torch.float16"):
+            cache.append(k, v)
+        with pytest.raises(RuntimeError, match="must be torch.float16"):
+            cache.extend([2, 0], k, v)
+    with pytest.raises(RuntimeError, match="cannot take -1 rows"):
+        cache.extend([2, -1], row(1), row(1))
+    assert cache.host_lengths == [1, 0] and cache.lengths.tolist() == [1, 0]
+    k = row(2)
+    cache.append(k, k)
+    cache.extend([1, 2], row(3), row(3))
+    assert cache.host_lengths == [3, 3] and torch.equal(cache.k[0, 1], k[0]) and torch.equal(cache.v[1, 0], k[1])

@@ -57,13 +57,22 @@ class SequenceCache:
         if len(more) != len(self.host_lengths):
             raise RuntimeError(f"expected {len(self.host_lengths)} sequences, got {len(more)}")
         for b, (have, add) in enumerate(zip(self.host_lengths, more)):
+            if add < 0:
+                raise RuntimeError(f"sequence {b} cannot take {add} rows")
             if have + add > self.capacity:
                 raise RuntimeError(f"cache of sequence {b} is full: {have} + {add} rows, capacity {self.capacity}")
+
+    def _fit(self, rows: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """k and v are that many rows of this cache's (index assignment would spread a single one)."""
+        for t, n in ((k, "k"), (v, "v")):
+            if t.shape != (rows, *self.k.shape[2:]) or t.dtype != self.k.dtype:
+                raise RuntimeError(f"{n} must be {self.k.dtype} {[rows, *self.k.shape[2:]]}, got {t.dtype} {list(t.shape)}")
 
     def extend(self, seq_lens: Sequence[int], k: torch.Tensor, v: torch.Tensor) -> None:
         """Append packed rows k, v [sum(seq_lens), Hkv, hd], seq_lens[b] of them to sequence b."""
         lens = [int(n) for n in seq_lens]
         self._room(lens)
+        self._fit(sum(lens), k, v)
         dev = self.k.device
         n = torch.tensor(lens, dtype=torch.int64)
         b = torch.repeat_interleave(torch.arange(len(lens)), n)
@@ -77,6 +86,7 @@ class SequenceCache:
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Append one row k, v [B, Hkv, hd] to every sequence."""
         self._room([1] * len(self.host_lengths))
+        self._fit(len(self.host_lengths), k, v)
         at = self.lengths.long()
         self.k[self._rows, at], self.v[self._rows, at] = k, v
         self.lengths += 1
