@@ -436,7 +436,7 @@ typedef struct ttj_cache_evict_args {
   void* k_out;                     /* [B, budget, num_kv_heads, head_dim]; aliases no input */
   void* v_out;
   float* weights_out;              /* [B, num_kv_heads, budget] */
-  int32_t* lengths_out;            /* [B] */
+  int32_t* lengths_out;            /* [B]; does not alias lengths */
   int32_t* positions_out;          /* [B, num_kv_heads, budget] */
   int64_t batch, capacity, num_kv_heads, head_dim, budget, recent;
   int64_t k_seq_stride, k_row_stride, k_head_stride;

@@ -1,9 +1,11 @@
 """What the serving entry points refuse, or leave as it was, before anything reaches a GPU."""
 
+import ctypes as C
+
 import pytest
 import torch
 
-from tiktok_techjam_2026_track3_b200 import CachedAttention, SequenceCache, SharedPrefix, ops
+from tiktok_techjam_2026_track3_b200 import CachedAttention, SequenceCache, SharedPrefix, _lib, ops
 
 
 def test_workspaces_that_would_be_used_are_dense_and_on_the_device():
@@ -98,3 +100,19 @@ def test_cache_rows_are_never_spread_over_sequences():
     cache.append(k, k)
     cache.extend([1, 2], row(3), row(3))
     assert cache.host_lengths == [3, 3] and torch.equal(cache.k[0, 1], k[0]) and torch.equal(cache.v[1, 0], k[1])
+
+
+def test_evict_refuses_to_write_the_lengths_it_reads():
+    """Every head's blocks read a sequence's length; the first one writes the new one."""
+    at = lambda i: (i + 1) << 40   # never dereferenced
+    a = _lib.CacheEvictArgs(
+        k_cache=at(0), v_cache=at(1), key_weights=at(2), lengths=at(3), k_out=at(4), v_out=at(5), weights_out=at(6),
+        positions_out=at(8), batch=2, capacity=8, num_kv_heads=2, head_dim=64, budget=4, recent=1,
+        k_seq_stride=1024, k_row_stride=128, k_head_stride=64, v_seq_stride=1024, v_row_stride=128, v_head_stride=64,
+        k_out_seq_stride=512, k_out_row_stride=128, k_out_head_stride=64, v_out_seq_stride=512, v_out_row_stride=128,
+        v_out_head_stride=64)
+    lib = _lib.load()
+    for out in (at(3), at(3) + 4, at(3) - 4):
+        a.lengths_out = out
+        assert lib.ttj_cache_evict(C.byref(a), None) == -1
+        assert b"lengths_out must not alias lengths" in lib.ttj_last_error()

@@ -228,6 +228,9 @@ int ttj_cache_evict(const ttj_cache_evict_args* a, ttj_stream_t stream) {
   const bool interleaved = a->k_out_seq_stride == a->v_out_seq_stride && a->k_out_row_stride == a->v_out_row_stride &&
                            a->k_out_head_stride == a->v_out_head_stride && gap >= row && gap + row <= a->k_out_row_stride;
   TTJ_CHECK_ARG(interleaved || !overlap(ko, vo), TTJ_ERR_INVALID_ARG, "k_out and v_out must not alias");
+  // One head's blocks write a sequence's new length while the others' still read it.
+  TTJ_CHECK_ARG(!overlap(span_of(a->lengths, 4, b, {}), span_of(a->lengths_out, 4, b, {})), TTJ_ERR_INVALID_ARG,
+                "lengths_out must not alias lengths");
   if (c > 0) {
     const Span ki = span_of(a->k_cache, 2, hd, {{b, a->k_seq_stride}, {c, a->k_row_stride}, {hkv, a->k_head_stride}});
     const Span vi = span_of(a->v_cache, 2, hd, {{b, a->v_seq_stride}, {c, a->v_row_stride}, {hkv, a->v_head_stride}});
