@@ -249,3 +249,56 @@ def test_repair_of_a_very_long_prompt_ends_no_wait(Hq, Hkv, hd):
     ops.check_device_status(q.device)
     assert torch.equal(out[n:], clean[n:]) and torch.equal(out[:n - 300], clean[:n - 300])
     check_rows(out, q, k, v, 0, [n - 200, n - 128, n - 71, n - 70, n - 1])
+
+
+# ------------------------------------------------------------------ right behind the kernels that write the inputs
+
+def step_chain(q, pk, pv, kc, vc, lens, w, budget):
+    """Eviction, then a decode step on what it wrote (lengths, rows and weights), then another."""
+    kept = ops.cache_evict(kc, vc, w, lens, budget, 3)
+    out, w1 = ops.shared_prefix_attn(q, pk, pv, kept.k, kept.v, kept.lengths, key_weights=kept.key_weights)
+    out2, w2 = ops.shared_prefix_attn(out, pk, pv, kept.k, kept.v, kept.lengths, key_weights=w1)
+    return kept.lengths, kept.positions, out, w1, out2, w2
+
+
+@pytest.mark.parametrize("B,P,C,Hq,Hkv,hd,budget", [(130, 513, 40, 32, 8, 128, 17), (33, 26001, 40, 32, 8, 128, 20),
+                                                    (300, 1025, 24, 16, 16, 64, 10), (140, 900, 25, 8, 2, 256, 11)])
+def test_decode_behind_the_kernels_that_write_its_inputs(B, P, C, Hq, Hkv, hd, budget):
+    """With the prefix on the tiles the caches' kernel starts without a wait of its own: chains of
+    calls on a side stream and in a graph, inputs changed in between, give what each step gives alone."""
+    sets = []
+    for seed in (1, 2):
+        q, pk, pv, kc, vc = decode_case(B, P, C, Hq, Hkv, hd, torch.bfloat16, seed)
+        lens = torch.tensor([(i * (3 + seed)) % (C + 1) for i in range(B)], dtype=torch.int32).cuda()
+        sets.append((q, pk, pv, kc, vc, lens, torch.rand(B, Hkv, C, generator=torch.Generator().manual_seed(seed)).cuda()))
+    want = []
+    for x in sets:
+        kept = ops.cache_evict(*x[3:5], x[6], x[5], budget, 3)
+        torch.cuda.synchronize()
+        out, w1 = ops.shared_prefix_attn(*x[:3], kept.k, kept.v, kept.lengths, key_weights=kept.key_weights)
+        torch.cuda.synchronize()
+        out2, w2 = ops.shared_prefix_attn(out, *x[1:3], kept.k, kept.v, kept.lengths, key_weights=w1)
+        torch.cuda.synchronize()
+        want.append((kept.lengths, kept.positions, out, w1, out2, w2))
+    held = tuple(t.clone() for t in sets[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    with torch.cuda.stream(side):
+        for i in range(20):
+            for h, t in zip(held, sets[i % 2]):
+                h.copy_(t)
+            got.append(step_chain(*held, budget))
+    side.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2])), i
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step_chain(*held, budget)
+    for i in range(10):
+        for h, t in zip(held, sets[i % 2]):
+            h.copy_(t)
+        graph.replay()
+        snap = [t.clone() for t in res]
+        assert all(torch.equal(a, b) for a, b in zip(snap, want[i % 2])), i
+    ops.check_device_status(side.device)
