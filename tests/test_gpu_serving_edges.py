@@ -302,3 +302,24 @@ def test_decode_behind_the_kernels_that_write_its_inputs(B, P, C, Hq, Hkv, hd, b
         snap = [t.clone() for t in res]
         assert all(torch.equal(a, b) for a, b in zip(snap, want[i % 2])), i
     ops.check_device_status(side.device)
+
+
+# ------------------------------------------------------------------ wide groups over caches larger than L2
+
+@pytest.mark.parametrize("Hq,Hkv,hd", [(32, 1, 128), (40, 2, 64)])
+def test_wide_groups_over_caches_larger_than_l2(Hq, Hkv, hd):
+    """A group of several row tiles reads its cache once per tile."""
+    B, C = 70, 8192 * 128 // (Hkv * hd)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    normal = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()
+    q, kc, vc = normal(B, Hq, hd), normal(B, C, Hkv, hd), normal(B, C, Hkv, hd)
+    none = kc.new_empty(0, Hkv, hd)
+    assert kc.numel() * 4 > 126 << 20
+    lengths = [C - 37 * b for b in range(B)]
+    w = torch.rand(B, Hkv, C, generator=gen, device="cuda")
+    out, new_w = ops.shared_prefix_attn(q, none, none, kc, vc, torch.tensor(lengths, dtype=torch.int32).cuda(), key_weights=w)
+    ref, bound, prob = decode_ref(q, none, none, kc, vc, lengths, hd ** -0.5)
+    check(out, ref, bound)
+    want = w.double() + prob
+    assert bool(((new_w.double() - want).abs() <= 4e-5 * prob + 2.0 ** -23 * want.abs()).all())
+    ops.check_device_status(q.device)

@@ -42,7 +42,7 @@ constexpr int kWarps = 4;
 // and 246.9 us for 128 caches of up to 4096 keys (245.2); 64 with half the step 43.5 and 248.1.
 constexpr int kJoinThreads = 128;
 constexpr int kWeightStep = 1024;  // cached keys per join block and step
-constexpr int64_t kL2Bytes = (int64_t)126 << 20;  // caches above it are read evict-first
+constexpr int64_t kL2Bytes = (int64_t)126 << 20;  // caches above it that are read once: evict-first
 constexpr int kMinSteps = 2;       // of a stretch
 // Beside the prefix kernel: up to kShareWaves times as many blocks as stay resident,
 // with stretches of at least kShareSteps (128 sequences behind 16384 keys with up to
@@ -96,7 +96,7 @@ struct LineParams {
   int batch, prefix, capacity, num_heads, head_groups, heads, group, hd;  // kv heads = head_groups * heads
   int prefix_units, prefix_row_tiles, cache_row_tiles, prefix_steps, pitch;
   int after_prefix;         // launched behind the prefix kernel of the same step
-  int large_caches;         // they are larger than L2
+  int large_caches;         // they are larger than L2 and read once
   float scale_log2;
 };
 
@@ -894,8 +894,12 @@ int launch_decode(const ttj_shared_prefix_attn_args& a, cudaStream_t stream) {
   p.pitch = c.pitch;
   p.after_prefix = c.prefix_tiles;
   // (33 sequences of 16 heads of 64, up to 2100 keys: 37.1 us a step, 39.9 without; 128
-  // of up to 2100: 92.9 and 101.4; 8 caches of 4 MB each, that fit: 18.3 and 16.4.)
-  p.large_caches = 4 * a.batch * a.capacity * a.num_kv_heads * a.head_dim > kL2Bytes;
+  // of up to 2100: 92.9 and 101.4; 8 caches of 4 MB each, that fit: 18.3 and 16.4.)  Not
+  // where a group takes several row tiles: each reads the cache again.  (Evict-first, with
+  // key weights: 32 heads over 1 of 128, 128 caches of 8192 rows 199 us against 188, 64 of
+  // 4096 58 against 62; 128 over 1, 32 of 8192 230 against 195; 24 over 2 of 64, 64 of 8192
+  // 123 against 115; without weights 0 to 5% slower.)
+  p.large_caches = c.cache_row_tiles == 1 && 4 * a.batch * a.capacity * a.num_kv_heads * a.head_dim > kL2Bytes;
   p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   // Without any cached or prefix key the line is empty, but the join reads `before`.
   const int blocks = std::max(c.blocks, 1);
