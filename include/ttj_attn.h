@@ -423,7 +423,9 @@ size_t ttj_shared_prefix_attn_workspace_size(int64_t batch, int64_t prefix_len, 
  *   key_weights_out[b,j,c] = key_weights[b,j,c] + sum over the group's heads of
  *                            this step's probability of cache row c
  * for c < lengths[b], and key_weights[b,j,c] for the rows beyond.  Cache rows
- * at and past the length may hold anything.
+ * at and past the length may hold anything.  A key that scores -inf weighs
+ * nothing; a row of such keys alone is as one without a key.  The workspace, of
+ * ttj_shared_prefix_attn_workspace_size() bytes, starts on any 16-byte boundary.
  */
 int ttj_shared_prefix_attn_fwd(const ttj_shared_prefix_attn_args* args, ttj_stream_t stream);
 

@@ -775,7 +775,7 @@ Cuts cuts_of(int64_t batch, int64_t prefix, int64_t capacity, int64_t num_heads,
   // the caches' blocks the SMs that their work is worth, by a key tile's ~1.9 us and
   // ~80 GB/s that an SM streams, caches taken as 0.6 full; as blocks of either end,
   // the line's take their place.  (Each kernel on the whole GPU in turn: 64 sequences
-  // behind 32768 keys 69.8 us a step, now 67.8.)  Steps of less than ~20 us in all gain
+  // behind 32768 keys 69.8 us a step, shared 67.8.)  Steps of less than ~20 us in all gain
   // nothing (33 sequences of up to 2100 keys: 47 us, shared 53).
   const double prefix_us = 1.9 * (double)(units * tiles);
   const double line_us = 0.6 * 4.0 * (double)(batch * kv_heads * c.cache_row_tiles) * (double)(capacity * hd) / 80e3;

@@ -44,12 +44,13 @@
 //                own TMEM columns; above, 4 warps per tile with 32 rows each, P
 //                written over S
 //
-// Bound by (16384 + 2049 tokens, 32 heads over 4 of 128: 2.07 ms, 1.08 PFLOP/s; 8 ragged
-// prompts of up to 2048, 16 heads of 64: 83 us, 0.56 PFLOP/s): at head_dim 128 a step
-// of two tiles takes ~3800 cycles, softmax 2050 plus its products and their hand-offs
+// Bound by (a call among others, 16384 + 2049 tokens, 32 heads over 4 of 128: 2.20 ms, 1.02
+// PFLOP/s; 8 ragged prompts of up to 2048, 16 heads of 64: 91 us, 0.51 PFLOP/s; replayed
+// as a graph 2.12 ms and 85 us): at head_dim 128 a step of two tiles takes ~3800 cycles, softmax 2050 plus its products and their hand-offs
 // 1740 per tile, alternating, against 2048 of the tensor pipe; at 64 the exponential
-// unit (60% busy) and the hand-offs.  Items of one or two key tiles (96 prompts of up
-// to 256 tokens: 67 us, 3.6 TB/s) take ~5 us each, their chain of barriers.
+// unit (62% busy) and the hand-offs.  Items of one or two key tiles (96 prompts of up
+// to 256 tokens: 74 us, 3.3 TB/s) take ~5 us each, their chain of barriers.  The head_dim-64
+// kernels spill 16 to 24 bytes of their 96 and 104 registers, the others none.
 #include <atomic>
 
 #include "attn_math.cuh"

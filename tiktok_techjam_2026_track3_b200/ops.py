@@ -561,7 +561,11 @@ def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
     ``key_weights`` (fp32 [B,Hkv,C]) gives new_key_weights, each cached key's weight
     plus this step's probabilities of that key summed over the group's heads, for
     ``cache_evict`` (the input is not written); ``return_lse`` gives the log of each
-    row's sum of exponentials, fp32 [B,Hq], -inf for a row without any key."""
+    row's sum of exponentials, fp32 [B,Hq], -inf for a row without any key.
+
+    A key that scores -inf weighs nothing, and a row of such keys alone is as one
+    without any.  ``workspace`` (contiguous, on q's device) is used if it is large
+    enough."""
     dt = _dtype_code(q)
     if q.dim() != 3 or prefix_k.dim() != 3 or k_cache.dim() != 4:
         raise RuntimeError("q must be [B,Hq,hd], prefix_k and prefix_v [P,Hkv,hd], k_cache and v_cache [B,C,Hkv,hd]")

@@ -161,7 +161,9 @@ class CachedAttention(nn.Module):
     def prefill(self, x: torch.Tensor, seq_lens: Sequence[int], cache: SequenceCache,
                 prefix: Optional[SharedPrefix] = None, plan: Optional[ops.PromptPlan] = None) -> torch.Tensor:
         """Prompts x [sum(seq_lens), d_model] of the cache's (empty) sequences: each token
-        attends the prefix and its own prompt up to itself."""
+        attends the prefix and its own prompt up to itself.  ``plan``, where the caller
+        has one, must be of these lengths.  Behind a prefix the two contexts are joined
+        as the operators return them, in x's dtype, and rounded once more."""
         if any(cache.host_lengths):
             raise RuntimeError("prefill starts sequences: the cache must be empty")
         lens = tuple(int(n) for n in seq_lens)
