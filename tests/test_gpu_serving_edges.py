@@ -323,3 +323,23 @@ def test_wide_groups_over_caches_larger_than_l2(Hq, Hkv, hd):
     want = w.double() + prob
     assert bool(((new_w.double() - want).abs() <= 4e-5 * prob + 2.0 ** -23 * want.abs()).all())
     ops.check_device_status(q.device)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,hd", HEADS)
+def test_an_infinite_value_without_weight_meets_later_ones(dt, Hq, Hkv, hd):
+    """A key that scores minus infinity and whose value is infinite: 0 times infinity is NaN, also
+    where a later token's infinity falls into the same column and tile."""
+    lens = [300, 130]
+    q, k, v = prompt_case(lens, Hq, Hkv, hd, DT[dt], hd + 2)
+    q = q.clone()
+    q[:300, :, 2] = q[:300, :, 2].abs() + 0.5
+    k[60, :, 2] = -math.inf
+    for at, col in ((60, 3), (100, 3), (61, 4), (100, 4), (270, 4), (290, 3)):
+        v[at, :, col] = math.inf
+    v[300 + 20, :, 4] = math.inf
+    v[300 + 90, :, 4] = math.inf
+    out = ops.prompt_attn(q, k, v, ops.PromptPlan(lens, Hq, Hkv, hd, q.device))
+    check_rows(out, q, k, v, 0, [0, 59, 60, 61, 62, 99, 100, 127, 128, 255, 256, 269, 270, 289, 290, 299])
+    check_rows(out, q, k, v, 300, [0, 19, 20, 89, 90, 129])
+    ops.check_device_status(q.device)

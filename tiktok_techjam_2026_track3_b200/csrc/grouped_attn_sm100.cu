@@ -231,9 +231,10 @@ __device__ __forceinline__ void box_free() {
 // Column c of an output depends on column c of V alone.  Per tile and column: the first
 // key whose value is NaN, +inf, -inf (among those its products read), and the last such
 // key that some row does not see.  A row is right where it sees that last key, or is NaN
-// by keys that it sees (a NaN, infinities of both signs); infinite by those alone it is
-// that infinity, unless its own sum is not finite (which a column of finite values
-// tells); else the block forms it again, the keys dealt out over the warps.
+// by keys that it sees (a NaN, infinities of both signs) or by its own sum (which a
+// column of finite values tells); infinite by those keys alone it is that infinity, if
+// their scores are finite for certain (`vast`); else the block forms it again, the keys
+// dealt out over the warps.
 // (One NaN at the end of 32768 tokens, 8 heads over 2 of 128: 46 ms; one warp per row, a
 // key after the other inside the softmax loop, took 540.)
 template <int HD>
@@ -248,6 +249,7 @@ struct Repair {
   static constexpr int kNone = 0x7fffffff;
   int first[3][HD], last[HD];                         // of NaN, +inf, -inf; of any
   int rows[kTile], count;                             // to be formed again
+  int vast;                                           // a key of such a value may score -inf: it weighs 0
   float m[kParts][kRows], l[kParts][kRows], o[kParts][kRows][HD];
 };
 
@@ -286,7 +288,8 @@ __device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x,
   };
   for (int k = k_lo; k <= k_hi; ++k) {
     const Seg s = seg_of<false, NT>(item_of(k), p);
-    const T* const kp = static_cast<const T*>(p.k) + s.k0 * p.k_row + s.kvh * p.k_head + piece * 8;
+    const T* const key = static_cast<const T*>(p.k) + s.k0 * p.k_row + s.kvh * p.k_head;
+    const T* const kp = key + piece * 8;
     const T* const vp = static_cast<const T*>(p.v) + s.k0 * p.v_row + s.kvh * p.v_head + piece * 8;
     for (int t = 0; t < NT; ++t) {
       const int keys = tile_keys<false>(s, t, p.positions);
@@ -297,7 +300,7 @@ __device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x,
         x.first[0][i] = x.first[1][i] = x.first[2][i] = R::kNone;
         x.last[i] = -1;
       }
-      if (tid == 0) x.count = 0;
+      if (tid == 0) x.count = x.vast = 0;
       repair_sync(R::kThreads);
       auto scan = [&](int from, int to, bool unseen) -> bool {
         constexpr int kStep = R::kThreads / R::kLanes, kAhead = 4;
@@ -318,6 +321,13 @@ __device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x,
             if (z == 0.f) continue;                       // all finite
             found = true;
             const int u = u0 + i * kStep;
+            for (int c = 0; c < p.hd && !*static_cast<volatile int*>(&x.vast); c += 8) {
+              float y[8];
+              unpack8<T>(__ldg(reinterpret_cast<const uint4*>(key + u * p.k_row + c)), y);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (!(fabsf(y[j]) < 1e30f)) x.vast = 1;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               if (e[j] - e[j] == 0.f) continue;
@@ -347,12 +357,15 @@ __device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x,
         form = __any_sync(0xffffffffu, form);
         infinite = __any_sync(0xffffffffu, infinite);
         finite = __reduce_max_sync(0xffffffffu, finite);
-        if (form || (infinite && finite < 0)) {
-          if (lane == 0) x.rows[atomicAdd(&x.count, 1)] = r;
-        } else if (infinite) {
+        if (!form && !infinite) continue;
+        if (!form && finite >= 0) {
           const uint16_t w = __ldcg(reinterpret_cast<const uint16_t*>(out + at * p.hd + finite));
           const float v = Pack<T>::unpack(w).x;
-          if (v != v) continue;
+          if (v != v) continue;                           // NaN altogether
+        }
+        if (form || finite < 0 || x.vast) {
+          if (lane == 0) x.rows[atomicAdd(&x.count, 1)] = r;
+        } else {
           for (int c = lane; c < p.hd; c += 32) {
             const int f0 = x.first[0][c], f1 = x.first[1][c], f2 = x.first[2][c];
             if (x.last[c] <= limit || f0 <= limit || (f1 <= limit) == (f2 <= limit)) continue;
@@ -430,7 +443,7 @@ __device__ __noinline__ void repair_items(const GroupedParams& p, Repair<HD>& x,
             v = fmaf(x.o[w][i][c], f, v);
           }
           v /= sum;
-          if (f1 <= lim || f2 <= lim) v = sum - sum != 0.f || sum == 0.f ? NAN : (f1 <= lim ? INFINITY : -INFINITY);
+          if (!x.vast && (f1 <= lim || f2 <= lim)) v = sum - sum != 0.f || sum == 0.f ? NAN : (f1 <= lim ? INFINITY : -INFINITY);
           put(row_index(r, pos, t, s, p), c, v);
         }
         repair_sync(R::kThreads);
